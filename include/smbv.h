@@ -481,6 +481,64 @@ int smbv_vjepa_forward(const smbv_vjepa_cfg* cfg, const smbv_vjepa_tensors* para
 int smbv_vjepa_backward(const smbv_vjepa_cfg* cfg, const smbv_vjepa_tensors* params, const smbv_vjepa_tensors* grads, const smbv_vjepa_io* io,
                         void* ws, size_t ws_bytes, void** events, int n_events, smbv_stream stream);
 
+/* ---- operators of a transformer block over long token sequences (ABI 3007) ------------------------------------------------------------------------
+ * Strides are in elements; channels are contiguous; dtype 0 = bf16, 1 = fp16 (and 2 = fp32 where noted).  None of these calls keeps state, forks onto another
+ * stream or synchronises: they may be captured into a graph and called from several host threads, each with workspaces of its own.  Outputs must not overlap
+ * inputs unless noted. */
+
+/* Windowed attention with sinks.  q [B, Sq, H, Dh], k / v [B, Sk, Hk, Dh], H a multiple of Hk (query head h reads key head h / (H / Hk)), Dh a multiple of 8 up
+ * to 128.  Query i of sequence b stands at position p = i + k_len - q_len and sees key j iff j < k_len, (right < 0 or j <= p + right) and (left < 0 or
+ * j >= p - left or j < sinks); left / right < 0: unbounded; right = 0: causal.  q_lens / k_lens: int32 [B] on the device, clamped to [0, Sq] / [0, Sk], NULL:
+ * Sq / Sk.  Rows that see nothing, padded rows included, get O = 0 and LSE = -inf and give no gradient; nothing past a length, and no key that no row of the
+ * call can see, takes part, whatever it holds.  o_lo (optional, o's strides): the residual of o's rounding, from which the backward forms rowsum(dO * O).
+ * lse: fp32 [B, H, Sq].  Pointers 16-byte aligned, strides multiples of 8.  The backward writes every element of dq, dk, dv. */
+typedef struct smbv_window_attn {
+  int struct_bytes, dtype, B, Sq, Sk, H, Hk, Dh, left, right, sinks;
+  float scale;                                /* > 0 */
+  const int *q_lens, *k_lens;
+  const void *q, *k, *v;
+  void *o, *o_lo; float *lse;                 /* forward: written; backward: read */
+  const void* d_o; void *dq, *dk, *dv;        /* backward only */
+  long long sq[3], sk[3], sv[3], so[3], sdo[3], sdq[3], sdk[3], sdv[3]; /* batch, row, head */
+} smbv_window_attn;
+size_t smbv_window_attention_fwd_workspace_bytes(const smbv_window_attn* a);
+int smbv_window_attention_fwd(const smbv_window_attn* a, void* ws, size_t ws_bytes, smbv_stream stream);
+size_t smbv_window_attention_bwd_workspace_bytes(const smbv_window_attn* a);
+int smbv_window_attention_bwd(const smbv_window_attn* a, void* ws, size_t ws_bytes, smbv_stream stream);
+
+/* Rotary positions with several axes.  q [B, S, H, Dh], k [B, S, Hk, Dh] (either may have no heads), dtype 0 / 1 / 2; the first 2 * pairs channels of a head
+ * turn, pair p by pos[axis(p)][b, s] * inv_freq[p], the axes owning consecutive runs of section[a] pairs; interleaved = 0: pairs (p, p + pairs), 1: (2p, 2p + 1).
+ * transpose: the inverse turn (the gradient's).  pos: int32 or int64 (pos64), strides spos = axis, batch, token.  inv_freq: fp32 [pairs].  qo / ko may be q / k
+ * themselves (same strides), otherwise the remaining channels are copied. */
+typedef struct smbv_rope_axes_cfg {
+  int struct_bytes, dtype, B, S, H, Hk, Dh, axes, section[4], interleaved, transpose, pos64;
+  const void *q, *k; void *qo, *ko;
+  long long sq[3], sk[3], sqo[3], sko[3];     /* batch, token, head */
+  const void* pos; long long spos[3];
+  const float* inv_freq;
+} smbv_rope_axes_cfg;
+int smbv_rope_axes(const smbv_rope_axes_cfg* a, smbv_stream stream);
+
+/* The norm behind a block, its gate, the scaled residual sum and the norm in front of the next block: x1 = res_scale * x + gate * post(h), y = pre(x1), over
+ * rows of d <= 8192.  post / pre: 0 none, 1 RMS norm, 2 LayerNorm; weights and biases fp32 [d] or NULL (1 / 0; their gradients then NULL too).  gate: fp32
+ * [rows / rows_per_gate, d], or NULL (1).  h, y, dy, dh have h_type, x, x1, dx1, dx have x_type (0 / 1 / 2; equal, or x_type fp32); ld*: row strides.
+ * stats: fp32 [rows, 4], written by the forward, read by the backward.  pre = 0: no y, no dy.  dx1 may be NULL (no gradient through x1).  rows = 0: nothing is
+ * written.  x1 may be x. */
+typedef struct smbv_gated_norm {
+  int struct_bytes, h_type, x_type, d, post, pre;
+  float eps, res_scale;
+  long long rows, rows_per_gate;
+  const void *h, *x;
+  const float *post_w, *post_b, *gate, *pre_w, *pre_b;
+  void *x1, *y; float* stats;
+  const void *dx1, *dy; void *dh, *dx;
+  float *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+  long long ldh, ldx, ldx1, ldy, lddx1, lddy, lddh, lddx;
+} smbv_gated_norm;
+int smbv_gated_norm_fwd(const smbv_gated_norm* a, smbv_stream stream);
+size_t smbv_gated_norm_bwd_workspace_bytes(const smbv_gated_norm* a);
+int smbv_gated_norm_bwd(const smbv_gated_norm* a, void* ws, size_t ws_bytes, smbv_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsmbv.so")
 MAX_LAYERS = 48
-ABI_MAJOR, ABI_MINOR_NEEDED = 3, 6  # include/smbv.h SMBV_ABI_MAJOR; the newest entry point these bindings call
+ABI_MAJOR, ABI_MINOR_NEEDED = 3, 7  # include/smbv.h SMBV_ABI_MAJOR; the newest entry point these bindings call
 
 c_f = C.c_void_p  # all device pointers travel as void*
 
@@ -111,6 +111,29 @@ class VjepaIO(C.Structure):
                                    "pred_out", "d_pred", "d_enc", "enc_pos")]
 
 
+c_ll3 = C.c_longlong * 3
+
+
+class WindowAttn(_Cfg):
+    _fields_ = [(n, C.c_int) for n in ("struct_bytes", "dtype", "B", "Sq", "Sk", "H", "Hk", "Dh", "left", "right", "sinks")] + \
+               [("scale", C.c_float)] + [(n, c_f) for n in ("q_lens", "k_lens", "q", "k", "v", "o", "o_lo", "lse", "d_o", "dq", "dk", "dv")] + \
+               [(n, c_ll3) for n in ("sq", "sk", "sv", "so", "sdo", "sdq", "sdk", "sdv")]
+
+
+class RopeAxesCfg(_Cfg):
+    _fields_ = [(n, C.c_int) for n in ("struct_bytes", "dtype", "B", "S", "H", "Hk", "Dh", "axes")] + [("section", C.c_int * 4)] + \
+               [(n, C.c_int) for n in ("interleaved", "transpose", "pos64")] + [(n, c_f) for n in ("q", "k", "qo", "ko")] + \
+               [(n, c_ll3) for n in ("sq", "sk", "sqo", "sko")] + [("pos", c_f), ("spos", c_ll3), ("inv_freq", c_f)]
+
+
+class GatedNorm(_Cfg):
+    _fields_ = [(n, C.c_int) for n in ("struct_bytes", "h_type", "x_type", "d", "post", "pre")] + [("eps", C.c_float), ("res_scale", C.c_float)] + \
+               [("rows", C.c_longlong), ("rows_per_gate", C.c_longlong)] + \
+               [(n, c_f) for n in ("h", "x", "post_w", "post_b", "gate", "pre_w", "pre_b", "x1", "y", "stats", "dx1", "dy", "dh", "dx", "dgate", "dpost_w",
+                                   "dpost_b", "dpre_w", "dpre_b")] + \
+               [(n, C.c_longlong) for n in ("ldh", "ldx", "ldx1", "ldy", "lddx1", "lddy", "lddh", "lddx")]
+
+
 _SIGS = {
     "smbv_version": (C.c_int, []),
     "smbv_last_error": (C.c_int, [C.c_char_p, C.c_size_t]),
@@ -169,6 +192,14 @@ _SIGS = {
     "smbv_encoder_backward": (C.c_int, [C.POINTER(EncoderCfg), C.POINTER(EncoderTensors), C.POINTER(EncoderTensors), C.POINTER(EncoderIO), c_f, c_f, C.c_size_t, c_f]),
     "smbv_encoder_hidden_states": (C.c_int, [C.POINTER(EncoderCfg), c_f, C.c_size_t, C.POINTER(C.c_void_p), C.c_int]),
     "smbv_mim_hidden_states": (C.c_int, [C.POINTER(MimCfg), c_f, C.c_size_t, C.POINTER(C.c_void_p), C.c_int]),
+    "smbv_window_attention_fwd_workspace_bytes": (C.c_size_t, [C.POINTER(WindowAttn)]),
+    "smbv_window_attention_fwd": (C.c_int, [C.POINTER(WindowAttn), c_f, C.c_size_t, c_f]),
+    "smbv_window_attention_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(WindowAttn)]),
+    "smbv_window_attention_bwd": (C.c_int, [C.POINTER(WindowAttn), c_f, C.c_size_t, c_f]),
+    "smbv_rope_axes": (C.c_int, [C.POINTER(RopeAxesCfg), c_f]),
+    "smbv_gated_norm_fwd": (C.c_int, [C.POINTER(GatedNorm), c_f]),
+    "smbv_gated_norm_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(GatedNorm)]),
+    "smbv_gated_norm_bwd": (C.c_int, [C.POINTER(GatedNorm), c_f, C.c_size_t, c_f]),
     "smbv_mim_workspace_bytes": (C.c_size_t, [C.POINTER(MimCfg)]),
     "smbv_mim_forward": (C.c_int, [C.POINTER(MimCfg), C.POINTER(MimTensors), C.POINTER(MimIO), c_f, C.c_size_t, c_f]),
     "smbv_mim_backward": (C.c_int, [C.POINTER(MimCfg), C.POINTER(MimTensors), C.POINTER(MimTensors), C.POINTER(MimIO), c_f, C.c_size_t,

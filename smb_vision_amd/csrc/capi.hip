@@ -2,6 +2,7 @@
 #include "smbv_common.h"
 #include "smbv_kernels.h"
 #include "block.h"
+#include "window_attention.h"
 #include "../../include/smbv.h"
 #include <cstdarg>
 #include <cstdio>
@@ -53,7 +54,7 @@ using namespace smbv;
 
 extern "C" {
 
-int smbv_version(void) { return 3006; }  // 3000: O_lo in smbv_attention_fwd / _bwd, attn_o_resid in the *_cfg structs; see include/smbv.h
+int smbv_version(void) { return 3007; }  // 3000: O_lo in smbv_attention_fwd / _bwd, attn_o_resid in the *_cfg structs; see include/smbv.h
 void smbv_debug_set_variant(int bits) { smbv::g_variant = bits; }
 int smbv_device_status(int clear) { return smbv::device_status(clear != 0); }
 int smbv_debug_pair_state(int op, smbv_stream stream) { return smbv::pair_state_debug(op, (hipStream_t)stream); }
@@ -251,5 +252,90 @@ int smbv_colsum_bf16(const smbv_bf16* X, int ld, int M, int N, float* out, void*
   return colsum_bf16(X, ld, M, N, out, 0, 0, 0, ws, ws_bytes, (hipStream_t)stream);
 }
 size_t smbv_colsum_workspace_bytes(int M, int N) { return colsum_workspace_bytes(M, N); }
+
+
+// windowed attention, rotary positions with several axes, gated norms: the C structs become the kernels' descriptions
+static bool win_desc(const smbv_window_attn* a, WinDesc& d, const char* what) {
+  if (!a || a->struct_bytes != (int)sizeof(smbv_window_attn)) { set_error("%s: struct_bytes does not match this library", what); return false; }
+  if (a->dtype < 0 || a->dtype > 1) { set_error("%s: dtype %d (0 bf16, 1 fp16)", what, a->dtype); return false; }
+  d = WinDesc{};
+  d.B = a->B; d.Sq = a->Sq; d.Sk = a->Sk; d.H = a->H; d.Hk = a->Hk; d.D = a->Dh; d.sinks = a->sinks; d.scale = a->scale;
+  d.G = a->Hk > 0 ? a->H / a->Hk : 0;
+  d.mG = d.G > 1 ? (unsigned)(((1ull << 32) + d.G - 1) / d.G) : 0;
+  const long long most = (long long)(a->Sq > 0 ? a->Sq : 0) + (a->Sk > 0 ? a->Sk : 0);   // (a window beyond both lengths is no bound)
+  d.left = a->left < 0 || a->left > most ? -1 : a->left;
+  d.right = a->right < 0 || a->right > most ? -1 : a->right;
+  d.q_lens = a->q_lens; d.k_lens = a->k_lens;
+  d.q = (const uint16_t*)a->q; d.k = (const uint16_t*)a->k; d.v = (const uint16_t*)a->v; d.g = (const uint16_t*)a->d_o;
+  d.o_in = (const uint16_t*)a->o; d.o_lo_in = (const uint16_t*)a->o_lo; d.o = (uint16_t*)a->o; d.o_lo = (uint16_t*)a->o_lo; d.lse = a->lse;
+  d.dq = (uint16_t*)a->dq; d.dk = (uint16_t*)a->dk; d.dv = (uint16_t*)a->dv;
+  const struct { WinStride* to; const long long* from; } st[] = {{&d.sq, a->sq}, {&d.sk, a->sk}, {&d.sv, a->sv}, {&d.so, a->so}, {&d.sg, a->sdo}, {&d.sdq, a->sdq}, {&d.sdk, a->sdk}, {&d.sdv, a->sdv}};
+  for (const auto& s : st) *s.to = WinStride{s.from[0], s.from[1], s.from[2]};
+  return true;
+}
+size_t smbv_window_attention_fwd_workspace_bytes(const smbv_window_attn* a) {
+  WinDesc d;
+  return win_desc(a, d, "smbv_window_attention_fwd_workspace_bytes") ? window_attention_fwd_workspace_bytes(d) : 0;
+}
+int smbv_window_attention_fwd(const smbv_window_attn* a, void* ws, size_t ws_bytes, smbv_stream stream) {
+  WinDesc d;
+  if (!win_desc(a, d, "smbv_window_attention_fwd")) return SMBV_ERR_ARG;
+  return window_attention_fwd(d, a->dtype, ws, ws_bytes, (hipStream_t)stream);
+}
+size_t smbv_window_attention_bwd_workspace_bytes(const smbv_window_attn* a) {
+  WinDesc d;
+  return win_desc(a, d, "smbv_window_attention_bwd_workspace_bytes") ? window_attention_bwd_workspace_bytes(d, a->dtype) : 0;
+}
+int smbv_window_attention_bwd(const smbv_window_attn* a, void* ws, size_t ws_bytes, smbv_stream stream) {
+  WinDesc d;
+  if (!win_desc(a, d, "smbv_window_attention_bwd")) return SMBV_ERR_ARG;
+  return window_attention_bwd(d, a->dtype, ws, ws_bytes, (hipStream_t)stream);
+}
+
+int smbv_rope_axes(const smbv_rope_axes_cfg* a, smbv_stream stream) {
+  if (!a || a->struct_bytes != (int)sizeof(smbv_rope_axes_cfg)) { set_error("smbv_rope_axes: struct_bytes does not match this library"); return SMBV_ERR_ARG; }
+  if (a->dtype < 0 || a->dtype > 2 || a->axes < 1 || a->axes > 4) { set_error("smbv_rope_axes: dtype %d (0 bf16, 1 fp16, 2 fp32), %d axes (1..4)", a->dtype, a->axes); return SMBV_ERR_ARG; }
+  RopeAxesDesc d = {};
+  d.B = a->B; d.S = a->S; d.H = a->H; d.Hk = a->Hk; d.D = a->Dh;
+  long long p = 0;
+  for (int i = 0; i < a->axes; i++) {
+    if (a->section[i] < 0) { set_error("smbv_rope_axes: a section of %d pairs", a->section[i]); return SMBV_ERR_ARG; }
+    p += a->section[i];
+    if (i < 3) d.end[i] = (int)std::min<long long>(p, 1 << 30);
+  }
+  d.P = (int)std::min<long long>(p, 1 << 30);
+  for (int i = a->axes; i < 4; i++) if (i - 1 < 3) d.end[i - 1] = d.P;
+  d.interleaved = a->interleaved != 0; d.transpose = a->transpose != 0; d.pos64 = a->pos64 != 0;
+  d.q = a->q; d.k = a->k; d.qo = a->qo; d.ko = a->ko;
+  d.copy = (a->H > 0 && a->q != a->qo) || (a->Hk > 0 && a->k != a->ko);
+  for (int i = 0; i < 3; i++) { d.sq[i] = a->sq[i]; d.sk[i] = a->sk[i]; d.sqo[i] = a->sqo[i]; d.sko[i] = a->sko[i]; }
+  d.pos = a->pos; d.pos_a = a->spos[0]; d.pos_b = a->spos[1]; d.pos_s = a->spos[2];
+  d.inv_freq = a->inv_freq;
+  return rope_axes(d, a->dtype, (hipStream_t)stream);
+}
+
+static bool gn_desc(const smbv_gated_norm* a, GatedNormDesc& d, const char* what) {
+  if (!a || a->struct_bytes != (int)sizeof(smbv_gated_norm)) { set_error("%s: struct_bytes does not match this library", what); return false; }
+  d = GatedNormDesc{};
+  d.rows = a->rows; d.rows_per_gate = a->rows_per_gate; d.d = a->d; d.post = a->post; d.pre = a->pre; d.eps = a->eps; d.res_scale = a->res_scale;
+  d.h = a->h; d.x = a->x; d.ldh = a->ldh; d.ldx = a->ldx;
+  d.post_w = a->post_w; d.post_b = a->post_b; d.gate = a->gate; d.pre_w = a->pre_w; d.pre_b = a->pre_b;
+  d.x1 = a->x1; d.y = a->y; d.ldx1 = a->ldx1; d.ldy = a->ldy; d.stats = a->stats;
+  d.dx1 = a->dx1; d.dy = a->dy; d.lddx1 = a->lddx1; d.lddy = a->lddy; d.dh = a->dh; d.dx = a->dx; d.lddh = a->lddh; d.lddx = a->lddx;
+  d.dgate = a->dgate; d.dpost_w = a->dpost_w; d.dpost_b = a->dpost_b; d.dpre_w = a->dpre_w; d.dpre_b = a->dpre_b;
+  return true;
+}
+int smbv_gated_norm_fwd(const smbv_gated_norm* a, smbv_stream stream) {
+  GatedNormDesc d;
+  return gn_desc(a, d, "smbv_gated_norm_fwd") ? gated_norm_fwd(d, a->h_type, a->x_type, (hipStream_t)stream) : SMBV_ERR_ARG;
+}
+size_t smbv_gated_norm_bwd_workspace_bytes(const smbv_gated_norm* a) {
+  GatedNormDesc d;
+  return gn_desc(a, d, "smbv_gated_norm_bwd_workspace_bytes") ? gated_norm_bwd_workspace_bytes(d) : 0;
+}
+int smbv_gated_norm_bwd(const smbv_gated_norm* a, void* ws, size_t ws_bytes, smbv_stream stream) {
+  GatedNormDesc d;
+  return gn_desc(a, d, "smbv_gated_norm_bwd") ? gated_norm_bwd(d, a->h_type, a->x_type, ws, ws_bytes, (hipStream_t)stream) : SMBV_ERR_ARG;
+}
 
 }  // extern "C"

@@ -1,0 +1,382 @@
+// The norm behind a block, its gate, the scaled residual sum and the norm in front of the next block as one pass, and its gradient:
+//     n = post(h) = hhat post_w + post_b,   x1 = res_scale x + gate n,   y = pre(x1) = xhat pre_w + pre_b
+// with hhat = (h - mean) / deviation (RMS norm: mean 0), the gate one row for `rows_per_gate` consecutive rows, and
+//     t  = dx1 + pre^T(dy),   dx = res_scale t,   dgate = sum t n,   dh = post^T(gate t),   dpost_w = sum gate t hhat,  dpre_w = sum dy xhat, ...
+//     norm^T(g) with z = w g:  (z - [LayerNorm: mean z] - hat mean(z hat)) / deviation
+// Bound by HBM: the forward reads h, x and writes x1, y; the backward reads dx1, dy, h, x (x1 is formed again from h and x in 32 bits rather than read back
+// rounded) and writes dh, dx.  A row lives in the registers of 1, 2 or 4 waves; sums and statistics are fp32, variances about the mean.
+// The parameters' gradients: every workgroup owns a run of rows and adds its rows' terms in registers; a second launch adds the workgroups' sums in a fixed
+// order (no float atomics: the result repeats bit for bit).
+#include "smbv_common.h"
+#include "smbv_kernels.h"
+#include <math.h>
+
+namespace smbv {
+
+template <class T, int V> struct __attribute__((aligned(V > 1 ? (sizeof(T) * V > 16 ? 16 : sizeof(T) * V) : sizeof(T)))) GnVec { T e[V]; };
+
+// the row's elements of this lane: NE of them in vectors of V, vector i at column (i LANES + lane) V; past the row's end zeros
+template <class T, int NE, int V, int LANES>
+__device__ __forceinline__ void gn_load(float (&f)[NE], const T* p, int lane, int d, bool on) {
+#pragma unroll
+  for (int i = 0; i < NE / V; i++) {
+    const int c = (i * LANES + lane) * V;
+    if (on && c < d) {
+      const GnVec<T, V> v = *(const GnVec<T, V>*)(p + c);
+#pragma unroll
+      for (int e = 0; e < V; e++) f[i * V + e] = (float)v.e[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++) f[i * V + e] = 0.f;
+    }
+  }
+}
+template <class T, int NE, int V, int LANES>
+__device__ __forceinline__ void gn_store(const float (&f)[NE], T* p, int lane, int d) {
+#pragma unroll
+  for (int i = 0; i < NE / V; i++) {
+    const int c = (i * LANES + lane) * V;
+    if (c < d) {
+      GnVec<T, V> v;
+#pragma unroll
+      for (int e = 0; e < V; e++) v.e[e] = (T)f[i * V + e];
+      *(GnVec<T, V>*)(p + c) = v;
+    }
+  }
+}
+template <int NE, int V, int LANES>
+__device__ __forceinline__ void gn_param(float (&f)[NE], const float* p, float none, int lane, int d) {
+  if (p) gn_load<float, NE, V, LANES>(f, p, lane, d, true);
+  else {
+#pragma unroll
+    for (int i = 0; i < NE; i++) f[i] = none;
+  }
+}
+// is register i of this lane inside the row
+template <int V, int LANES> __device__ __forceinline__ bool gn_in(int i, int lane, int d) { return ((i / V) * LANES + lane) * V < d; }
+
+// sums over a row's K waves; every wave of the workgroup calls it the same number of times (two alternating slots: one barrier a call)
+template <int K, int N>
+struct GnReduce {
+  float* slots;  // LDS [2][4 waves][N]
+  int flip;
+  __device__ __forceinline__ void operator()(float (&s)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) s[i] = wave_sum(s[i]);
+    if constexpr (K > 1) {
+      const int w = threadIdx.x >> 6, l = threadIdx.x & 63, w0 = w & ~(K - 1);
+      float* at = slots + flip * 4 * N;
+      if (l == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i++) at[w * N + i] = s[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        s[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; k++) s[i] += at[(w0 + k) * N + i];
+      }
+      flip ^= 1;
+    }
+  }
+};
+
+template <int NE, int V, int LANES, int K>
+__device__ __forceinline__ void gn_stats(const float (&f)[NE], int kind, int lane, int d, float eps, float& mu, float& rs, GnReduce<K, 2>& red) {
+  mu = 0.f;
+  if (kind == 2) {
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NE; i++) s[0] += f[i];
+    red(s);
+    mu = s[0] / d;
+  }
+  float q[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NE; i++) {
+    const float c = gn_in<V, LANES>(i, lane, d) ? f[i] - mu : 0.f;
+    q[0] += c * c;
+  }
+  red(q);
+  rs = 1.0f / sqrtf(q[0] / d + eps);
+}
+
+template <class TH, class TX, int NE, int V, int K>
+__global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GatedNormDesc d) {
+  constexpr int LANES = 64 * K, TEAMS = 4 / K;
+  __shared__ float slots[2 * 4 * 2];
+  const int lane = threadIdx.x & (LANES - 1), team = threadIdx.x / LANES;
+  const long long row = (long long)blockIdx.x * TEAMS + team;
+  const bool on = row < d.rows;
+  GnReduce<K, 2> red{slots, 0};
+  float h[NE], x[NE], w[NE];
+  gn_load<TH, NE, V, LANES>(h, (const TH*)d.h + row * d.ldh, lane, d.d, on);
+  gn_load<TX, NE, V, LANES>(x, (const TX*)d.x + row * d.ldx, lane, d.d, on);
+  float mu = 0.f, rs = 1.f;
+  if (d.post) {
+    gn_stats<NE, V, LANES, K>(h, d.post, lane, d.d, d.eps, mu, rs, red);
+    float b[NE];
+    gn_param<NE, V, LANES>(w, d.post_w, 1.f, lane, d.d);
+    gn_param<NE, V, LANES>(b, d.post_b, 0.f, lane, d.d);
+#pragma unroll
+    for (int i = 0; i < NE; i++) h[i] = (h[i] - mu) * rs * w[i] + b[i];
+  }
+  if (d.gate) {
+    gn_param<NE, V, LANES>(w, d.gate + (on ? row / d.rows_per_gate : 0) * d.d, 1.f, lane, d.d);
+#pragma unroll
+    for (int i = 0; i < NE; i++) h[i] *= w[i];
+  }
+#pragma unroll
+  for (int i = 0; i < NE; i++) x[i] = gn_in<V, LANES>(i, lane, d.d) ? __builtin_fmaf(d.res_scale, x[i], h[i]) : 0.f;
+  if (on) gn_store<TX, NE, V, LANES>(x, (TX*)d.x1 + row * d.ldx1, lane, d.d);
+  float mx = 0.f, rx = 1.f;
+  if (d.pre) {
+    gn_stats<NE, V, LANES, K>(x, d.pre, lane, d.d, d.eps, mx, rx, red);
+    float b[NE];
+    gn_param<NE, V, LANES>(w, d.pre_w, 1.f, lane, d.d);
+    gn_param<NE, V, LANES>(b, d.pre_b, 0.f, lane, d.d);
+#pragma unroll
+    for (int i = 0; i < NE; i++) x[i] = (x[i] - mx) * rx * w[i] + b[i];
+    if (on) gn_store<TH, NE, V, LANES>(x, (TH*)d.y + row * d.ldy, lane, d.d);
+  }
+  if (on && lane == 0) *(f32x4*)(d.stats + 4 * row) = (f32x4){mu, rs, mx, rx};
+}
+
+// workspace of the backward: sums of C workgroups, [C][d] each: pre_w | pre_b | post_w | post_b, then the gate's, [C + gates][d]
+struct GnPart { float* base; int C; long long chunk; };
+
+template <class TH, class TX, int NE, int V, int K>
+__global__ __launch_bounds__(256, NE > 16 ? 1 : 2) void gated_norm_bwd_kernel(GatedNormDesc d, GnPart part) {
+  constexpr int LANES = 64 * K, TEAMS = 4 / K;
+  __shared__ float slots[2 * 4 * 2];
+  __shared__ float fold[TEAMS > 1 ? (TEAMS - 1) * LANES * NE : 1];
+  const int lane = threadIdx.x & (LANES - 1), team = threadIdx.x / LANES;
+  GnReduce<K, 2> red{slots, 0};
+  const long long c0 = blockIdx.x * part.chunk, c1 = c0 + part.chunk < d.rows ? c0 + part.chunk : d.rows;
+  const bool per_row = d.gate && d.rows_per_gate == 1;
+  float sw[NE], sb[NE], qw[NE], qb[NE], sg[NE];  // pre_w, pre_b, post_w, post_b, gate
+#pragma unroll
+  for (int i = 0; i < NE; i++) { sw[i] = 0.f; sb[i] = 0.f; qw[i] = 0.f; qb[i] = 0.f; }
+  // the teams' sums into one row of the workspace (team 0 writes)
+  auto flush = [&](float (&s)[NE], float* out) __attribute__((always_inline)) {
+    if constexpr (TEAMS > 1) {
+      __syncthreads();
+      if (team > 0) {
+#pragma unroll
+        for (int i = 0; i < NE; i++) fold[((team - 1) * NE + i) * LANES + lane] = s[i];
+      }
+      __syncthreads();
+      if (team == 0) {
+        for (int k = 0; k < TEAMS - 1; k++)
+#pragma unroll
+          for (int i = 0; i < NE; i++) s[i] += fold[(k * NE + i) * LANES + lane];
+      }
+    }
+    if (team == 0) gn_store<float, NE, V, LANES>(s, out, lane, d.d);
+  };
+  const long long rpg = d.gate && !per_row ? d.rows_per_gate : d.rows;
+  for (long long s0 = c0; s0 < c1;) {   // runs of rows with one gate
+    const long long g = s0 / rpg, s1 = (g + 1) * rpg < c1 ? (g + 1) * rpg : c1;
+    float gt[NE];
+    if (!per_row) gn_param<NE, V, LANES>(gt, d.gate ? d.gate + g * d.d : nullptr, 1.f, lane, d.d);
+#pragma unroll
+    for (int i = 0; i < NE; i++) sg[i] = 0.f;
+    for (long long base = s0; base < s1; base += TEAMS) {
+      const long long row = base + team;
+      const bool on = row < s1;
+      f32x4 st = {0.f, 0.f, 0.f, 0.f};
+      if (on) st = *(const f32x4*)(d.stats + 4 * row);
+      float h[NE], x[NE], t[NE], dy[NE], w[NE];
+      gn_load<TH, NE, V, LANES>(h, (const TH*)d.h + row * d.ldh, lane, d.d, on);
+      gn_load<TX, NE, V, LANES>(x, (const TX*)d.x + row * d.ldx, lane, d.d, on);
+      gn_load<TX, NE, V, LANES>(t, (const TX*)d.dx1 + row * d.lddx1, lane, d.d, on && d.dx1);
+      if (per_row) gn_param<NE, V, LANES>(gt, on ? d.gate + row * d.d : nullptr, 1.f, lane, d.d);
+      float n[NE];
+      gn_param<NE, V, LANES>(w, d.post_w, 1.f, lane, d.d);
+      float b[NE];
+      gn_param<NE, V, LANES>(b, d.post_b, 0.f, lane, d.d);
+#pragma unroll
+      for (int i = 0; i < NE; i++) {
+        if (d.post) h[i] = gn_in<V, LANES>(i, lane, d.d) ? (h[i] - st[0]) * st[1] : 0.f;   // hhat
+        n[i] = d.post ? h[i] * w[i] + b[i] : h[i];
+      }
+      if (d.pre) {
+        gn_load<TH, NE, V, LANES>(dy, (const TH*)d.dy + row * d.lddy, lane, d.d, on);
+        float s[2] = {0.f, 0.f}, pw[NE];
+        gn_param<NE, V, LANES>(pw, d.pre_w, 1.f, lane, d.d);
+#pragma unroll
+        for (int i = 0; i < NE; i++) {
+          x[i] = gn_in<V, LANES>(i, lane, d.d) ? (__builtin_fmaf(d.res_scale, x[i], gt[i] * n[i]) - st[2]) * st[3] : 0.f;   // xhat
+          sw[i] += dy[i] * x[i];
+          sb[i] += dy[i];
+          dy[i] *= pw[i];
+          s[0] += dy[i] * x[i];
+          s[1] += dy[i];
+        }
+        red(s);
+        const float m1 = s[0] / d.d, m0 = d.pre == 2 ? s[1] / d.d : 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; i++) t[i] += gn_in<V, LANES>(i, lane, d.d) ? (dy[i] - m0 - x[i] * m1) * st[3] : 0.f;
+      }
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NE; i++) {
+        x[i] = t[i] * d.res_scale;                 // dx
+        const float tn = t[i] * n[i], u = t[i] * gt[i];
+        n[i] = tn;                                 // this row's dgate
+        sg[i] += tn;
+        qw[i] += u * h[i];
+        qb[i] += u;
+        t[i] = d.post ? u * w[i] : u;
+        s[0] += t[i] * h[i];
+        s[1] += t[i];
+      }
+      if (on) gn_store<TX, NE, V, LANES>(x, (TX*)d.dx + row * d.lddx, lane, d.d);
+      if (on && per_row) gn_store<float, NE, V, LANES>(n, d.dgate + row * d.d, lane, d.d);
+      if (d.post) {
+        red(s);
+        const float m1 = s[0] / d.d, m0 = d.post == 2 ? s[1] / d.d : 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; i++) t[i] = (t[i] - m0 - h[i] * m1) * st[1];
+      }
+      if (on) gn_store<TH, NE, V, LANES>(t, (TH*)d.dh + row * d.lddh, lane, d.d);
+    }
+    // this workgroup's share of gate g: slot (workgroup + gate) is its own (both only ever grow)
+    if (d.gate && !per_row) flush(sg, s0 == g * rpg && s1 == (g + 1) * rpg ? d.dgate + g * d.d : part.base + ((long long)4 * part.C + blockIdx.x + g) * d.d);
+    s0 = s1;
+  }
+  if (d.dpre_w) flush(sw, part.base + (long long)blockIdx.x * d.d);
+  if (d.dpre_b) flush(sb, part.base + ((long long)part.C + blockIdx.x) * d.d);
+  if (d.dpost_w) flush(qw, part.base + ((long long)2 * part.C + blockIdx.x) * d.d);
+  if (d.dpost_b) flush(qb, part.base + ((long long)3 * part.C + blockIdx.x) * d.d);
+}
+
+// sums of the workgroups, in their order: blockIdx.y 0..3 the four parameter vectors, the others the gate rows; 64 columns a block, 4 waves share the workgroups
+__global__ __launch_bounds__(256) void gated_norm_finish_kernel(GatedNormDesc d, GnPart part, long long gates) {
+  __shared__ float fold[4][64];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + l;
+  auto sum = [&](const float* from, long long lo, long long hi, float* out) {
+    float s = 0.f;
+    if (col < d.d)
+      for (long long i = lo + w; i < hi; i += 4) s += from[i * d.d + col];
+    fold[w][l] = s;
+    __syncthreads();
+    if (w == 0 && col < d.d) out[col] = (fold[0][l] + fold[1][l]) + (fold[2][l] + fold[3][l]);
+    __syncthreads();
+  };
+  if (blockIdx.y < 4) {
+    float* out = blockIdx.y == 0 ? d.dpre_w : blockIdx.y == 1 ? d.dpre_b : blockIdx.y == 2 ? d.dpost_w : d.dpost_b;
+    if (out) sum(part.base + (long long)blockIdx.y * part.C * d.d, 0, part.C, out);
+    return;
+  }
+  for (long long g = blockIdx.y - 4; g < gates; g += gridDim.y - 4) {
+    const long long r0 = g * d.rows_per_gate, r1 = r0 + d.rows_per_gate, lo = r0 / part.chunk, hi = (r1 - 1) / part.chunk + 1;
+    // (one workgroup that held all of a gate's rows has written the sum itself)
+    if (hi - lo > 1) sum(part.base + ((long long)4 * part.C + g) * d.d, lo, hi, d.dgate + g * d.d);
+  }
+}
+
+static int gn_teams(int d) { return d <= 1024 ? 4 : d <= 2048 ? 2 : 1; }
+static GnPart gn_part(const GatedNormDesc& d, void* ws) {
+  // two workgroups a CU; a run of rows is a whole number of rounds of the workgroup's teams
+  const int teams = gn_teams(d.d);
+  GnPart p;
+  p.chunk = (((d.rows + 511) / 512 + teams - 1) / teams) * teams;
+  p.C = (int)((d.rows + p.chunk - 1) / p.chunk);
+  p.base = (float*)ws;
+  return p;
+}
+static long long gn_gates(const GatedNormDesc& d) { return d.gate && d.rows_per_gate > 1 ? d.rows / d.rows_per_gate : 0; }
+
+size_t gated_norm_bwd_workspace_bytes(const GatedNormDesc& d) {
+  if (d.rows <= 0 || d.d <= 0) return 256;
+  const GnPart p = gn_part(d, nullptr);
+  return ((size_t)5 * p.C + gn_gates(d)) * d.d * sizeof(float) + 256;
+}
+
+static int gn_check(const GatedNormDesc& d, int ht, int xt, bool bwd, const char* what, bool& wide) {
+  if (d.rows < 0 || d.rows >= (1ll << 31) || d.d <= 0 || d.d > 8192) { set_error("%s: %lld rows of %d (rows up to 8192 wide)", what, d.rows, d.d); return SMBV_ERR_SHAPE; }
+  if (ht < 0 || ht > 2 || xt < 0 || xt > 2 || (xt != ht && xt != 2)) { set_error("%s: the residual stream has the block's type or fp32", what); return SMBV_ERR_ARG; }
+  if (d.post < 0 || d.post > 2 || d.pre < 0 || d.pre > 2) { set_error("%s: unknown norm", what); return SMBV_ERR_ARG; }
+  if ((!d.post && (d.post_w || d.post_b)) || (!d.pre && (d.pre_w || d.pre_b))) { set_error("%s: a weight or bias without its norm", what); return SMBV_ERR_ARG; }
+  if (d.gate && (d.rows_per_gate <= 0 || d.rows % d.rows_per_gate)) { set_error("%s: %lld rows are not whole groups of %lld", what, d.rows, d.rows_per_gate); return SMBV_ERR_SHAPE; }
+  if (!(d.eps >= 0.f)) { set_error("%s: eps must not be negative", what); return SMBV_ERR_ARG; }
+  if (d.rows == 0) return SMBV_OK;
+  if (!d.h || !d.x || !d.stats || (!bwd && (!d.x1 || (d.pre && !d.y)))) { set_error("%s: null operand", what); return SMBV_ERR_ARG; }
+  if (bwd && (!d.dh || !d.dx || (d.pre && !d.dy) || (!d.pre && !d.dx1) || (d.gate && !d.dgate))) { set_error("%s: null operand", what); return SMBV_ERR_ARG; }
+  if (bwd && ((d.dpost_w && !d.post_w) || (d.dpost_b && !d.post_b) || (d.dpre_w && !d.pre_w) || (d.dpre_b && !d.pre_b) || (d.dgate && !d.gate))) { set_error("%s: the gradient of an absent parameter", what); return SMBV_ERR_ARG; }
+  const long long lds[] = {d.ldh, d.ldx, d.ldx1, d.ldy, d.lddx1, d.lddy, d.lddh, d.lddx};
+  const void* ps[] = {d.h, d.x, d.x1, d.y, d.dx1, d.dy, d.dh, d.dx};
+  const int types[] = {ht, xt, xt, ht, xt, ht, ht, xt};
+  long long bits = d.d;
+  uintptr_t addr = 0;
+  for (int i = 0; i < 8; i++) {
+    if (!ps[i]) continue;
+    if ((uintptr_t)ps[i] & (types[i] == 2 ? 3 : 1)) { set_error("%s: alignment", what); return SMBV_ERR_ALIGN; }
+    if (lds[i] < d.d) { set_error("%s: a row stride of %lld for rows of %d", what, lds[i], d.d); return SMBV_ERR_SHAPE; }
+    bits |= lds[i];
+    addr |= (uintptr_t)ps[i];
+  }
+  const void* fs[] = {d.post_w, d.post_b, d.gate, d.pre_w, d.pre_b, d.dgate, d.dpost_w, d.dpost_b, d.dpre_w, d.dpre_b};
+  for (const void* p : fs) {
+    if ((uintptr_t)p & 3) { set_error("%s: alignment", what); return SMBV_ERR_ALIGN; }
+    addr |= (uintptr_t)p;
+  }
+  if ((uintptr_t)d.stats & 15) { set_error("%s: stats must be 16-byte aligned", what); return SMBV_ERR_ALIGN; }
+  wide = (bits & 7) == 0 && (addr & 15) == 0;
+  return SMBV_OK;
+}
+
+// waves a row and elements a lane by the row's width: as few waves as hold it in 16 registers an operand (32 beyond 4096)
+#define GN_SHAPES(GO)                 \
+  if (d.d <= 512) GO(8, 1)            \
+  else if (d.d <= 1024) GO(16, 1)     \
+  else if (d.d <= 2048) GO(16, 2)     \
+  else if (d.d <= 4096) GO(16, 4)     \
+  else GO(32, 4)
+
+template <class TH, class TX>
+static void gn_fwd(const GatedNormDesc& d, bool wide, hipStream_t st) {
+  const int teams = gn_teams(d.d);
+  const dim3 grid((unsigned)((d.rows + teams - 1) / teams)), blk(256);
+#define GO(NE, K) { if (wide) hipLaunchKernelGGL((gated_norm_fwd_kernel<TH, TX, NE, 8, K>), grid, blk, 0, st, d); \
+                    else hipLaunchKernelGGL((gated_norm_fwd_kernel<TH, TX, NE, 1, K>), grid, blk, 0, st, d); }
+  GN_SHAPES(GO)
+#undef GO
+}
+template <class TH, class TX>
+static void gn_bwd(const GatedNormDesc& d, bool wide, const GnPart& part, hipStream_t st) {
+  const dim3 grid(part.C), blk(256);
+#define GO(NE, K) { if (wide) hipLaunchKernelGGL((gated_norm_bwd_kernel<TH, TX, NE, 8, K>), grid, blk, 0, st, d, part); \
+                    else hipLaunchKernelGGL((gated_norm_bwd_kernel<TH, TX, NE, 1, K>), grid, blk, 0, st, d, part); }
+  GN_SHAPES(GO)
+#undef GO
+}
+#define GN_TYPES(FN, ...)                                                       \
+  if (ht == 0) { if (xt == 0) FN<__bf16, __bf16>(__VA_ARGS__); else FN<__bf16, float>(__VA_ARGS__); }            \
+  else if (ht == 1) { if (xt == 1) FN<_Float16, _Float16>(__VA_ARGS__); else FN<_Float16, float>(__VA_ARGS__); } \
+  else FN<float, float>(__VA_ARGS__);
+
+int gated_norm_fwd(const GatedNormDesc& d, int ht, int xt, hipStream_t st) {
+  bool wide = false;
+  if (int rc = gn_check(d, ht, xt, false, "gated_norm_fwd", wide)) return rc;
+  if (d.rows == 0) return SMBV_OK;
+  GN_TYPES(gn_fwd, d, wide, st)
+  return check_launch("gated_norm_fwd");
+}
+
+int gated_norm_bwd(const GatedNormDesc& d, int ht, int xt, void* ws, size_t ws_bytes, hipStream_t st) {
+  bool wide = false;
+  if (int rc = gn_check(d, ht, xt, true, "gated_norm_bwd", wide)) return rc;
+  if (d.rows == 0) return SMBV_OK;
+  const size_t need = gated_norm_bwd_workspace_bytes(d);
+  if (!ws || ws_bytes < need || ((uintptr_t)ws & 255)) { set_error("gated_norm_bwd: workspace short or not 256-byte aligned (%zu < %zu)", ws_bytes, need); return SMBV_ERR_WORKSPACE; }
+  const GnPart part = gn_part(d, ws);
+  GN_TYPES(gn_bwd, d, wide, part, st)
+  const long long gates = gn_gates(d);
+  hipLaunchKernelGGL(gated_norm_finish_kernel, dim3((d.d + 63) / 64, 4 + (unsigned)std::min<long long>(gates, 512)), dim3(256), 0, st, d, part, gates);
+  return check_launch("gated_norm_bwd");
+}
+
+}  // namespace smbv

@@ -179,4 +179,33 @@ int scatter_rows_idx_f32(const float* src, float* dst, const int* idx, long nidx
 int fill_rows_idx_f32(float* dst, const float* vec, const int* idx, long nidx, int per_batch, long dst_batch_rows, int D, hipStream_t st);
 int map_copy_f32(float* dst, const float* src, size_t n, long grp_in, long grp_out, hipStream_t st);
 
+// rotary positions with several axes (rope_axes.hip); dtype 0 bf16, 1 fp16, 2 fp32; strides in elements (batch, token, head)
+struct RopeAxesDesc {
+  int B, S, H, Hk, D, P;
+  int end[3];                    // running ends of the axes' runs of pairs (P where there is no further axis)
+  int interleaved, transpose, copy, pos64;
+  const void *q, *k; void *qo, *ko;
+  long long sq[3], sk[3], sqo[3], sko[3];
+  const void* pos; long long pos_a, pos_b, pos_s;
+  const float* inv_freq;
+};
+int rope_axes(const RopeAxesDesc& d, int dtype, hipStream_t st);
+
+// norm behind a block, gate, scaled residual sum, norm in front of the next block (gated_norm.hip); types: 0 bf16, 1 fp16, 2 fp32; norms: 0 none, 1 RMS, 2 LayerNorm
+struct GatedNormDesc {
+  long long rows, rows_per_gate;  // rows_per_gate: consecutive rows that share a row of the gate
+  int d, post, pre;
+  float eps, res_scale;
+  const void *h, *x; long long ldh, ldx;
+  const float *post_w, *post_b, *gate, *pre_w, *pre_b;
+  void *x1, *y; long long ldx1, ldy;      // forward
+  float* stats;                           // [rows, 4]: mean and 1 / deviation of h, of x1
+  const void *dx1, *dy; long long lddx1, lddy;  // backward
+  void *dh, *dx; long long lddh, lddx;
+  float *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+};
+int gated_norm_fwd(const GatedNormDesc& d, int h_type, int x_type, hipStream_t st);
+size_t gated_norm_bwd_workspace_bytes(const GatedNormDesc& d);
+int gated_norm_bwd(const GatedNormDesc& d, int h_type, int x_type, void* ws, size_t ws_bytes, hipStream_t st);
+
 }  // namespace smbv

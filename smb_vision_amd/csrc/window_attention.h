@@ -1,0 +1,121 @@
+// Windowed attention with sinks: what the forward and the backward share - the operator's description, the geometry of a window and the LDS image.
+//
+// Query row i of sequence b stands at key position p = i + klen_b - qlen_b (the queries are the LAST rows of their sequence: a training batch has
+// qlen = klen, an appended piece or a single token has qlen < klen).  It sees key j iff
+//     j < klen_b,   right < 0 or j <= p + right,   left < 0 or j >= p - left or j < sinks.
+//     O_i = sum_j P_ij V_j,  P_ij = exp(scale Q_i K_j - LSE_i);  a row that sees nothing has O_i = 0, LSE_i = -inf and gives no gradient.
+//
+// Heads are grouped: H = G Hk query heads, head h reads key head h / G.  The kernels work on ROWS r = i G + g (query i, head hk G + g): the G heads of a
+// group share every key tile that is fetched, and a tile of R rows spans only R / G positions, so its window is narrower.
+#pragma once
+#include "smbv_common.h"
+#include "smbv_kernels.h"
+
+namespace smbv {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+struct ElBf16 {
+  using v8 = bf16x8;
+  using e = __bf16;
+  static constexpr bool half = false;
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+struct ElF16 {
+  using v8 = f16x8;
+  using e = _Float16;
+  static constexpr bool half = true;
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <class E> __device__ __forceinline__ float el_f(uint16_t u) { return (float)__builtin_bit_cast(typename E::e, u); }
+template <class E> __device__ __forceinline__ uint16_t el_u(float f) { return __builtin_bit_cast(uint16_t, (typename E::e)f); }
+template <class E> __device__ __forceinline__ unsigned el_pack(float lo, float hi) { return (unsigned)el_u<E>(lo) | ((unsigned)el_u<E>(hi) << 16); }
+
+struct WinStride { long long b, r, h; };  // elements between batches, rows, heads (channels are contiguous)
+
+struct WinDesc {
+  int B, Sq, Sk, H, Hk, G, D, left, right, sinks;
+  unsigned mG;  // ceil(2^32 / G): r / G by multiplication, exact while r G < 2^32 (checked on the host)
+  float scale;
+  const int *q_lens, *k_lens;  // per sequence; null = Sq / Sk
+  const uint16_t *q, *k, *v, *o_in, *o_lo_in, *g;
+  uint16_t *o, *o_lo, *dq, *dk, *dv;
+  float *lse, *delta;
+  WinStride sq, sk, sv, so, sg, sdq, sdk, sdv;
+};
+
+struct WinSeq { int klen, qlen, shift; };
+__device__ __forceinline__ WinSeq win_seq(const WinDesc& d, int b) {
+  WinSeq s;
+  s.klen = d.k_lens ? max(0, min(d.k_lens[b], d.Sk)) : d.Sk;
+  s.qlen = d.q_lens ? max(0, min(d.q_lens[b], d.Sq)) : d.Sq;
+  s.shift = s.klen - s.qlen;
+  return s;
+}
+__device__ __forceinline__ int win_div(const WinDesc& d, int r) { return d.G == 1 ? r : (int)__umulhi((unsigned)r, d.mG); }
+
+// The keys that the queries [i0, i1) can see between them, as ONE run of n: first the ns sinks that lie in front of the window, then the window [lo, hi).
+// Sinks therefore cost ns keys of the first tile, not a tile of their own.  Key number of run index u: u < ns ? u : u + jump.
+struct WinKeys { int ns, hi, n, jump; };
+__device__ __forceinline__ WinKeys win_keys(const WinDesc& d, const WinSeq& s, int i0, int i1) {
+  WinKeys w;
+  w.hi = d.right < 0 ? s.klen : max(0, min(s.klen, i1 - 1 + s.shift + d.right + 1));
+  int lo = d.left < 0 ? 0 : max(0, min(w.hi, i0 + s.shift - d.left));
+  w.ns = min(d.sinks, w.hi);
+  if (w.ns >= lo) { w.ns = 0; lo = 0; }
+  w.n = i1 > i0 ? w.ns + w.hi - lo : 0;
+  w.jump = lo - w.ns;
+  return w;
+}
+// what one query sees: keys [0, sinks) and [lo, ...) up to hi (inclusive)
+struct WinRow { int lo, hi; };
+__device__ __forceinline__ WinRow win_row(const WinDesc& d, const WinSeq& s, int i) {
+  const int p = i + s.shift;
+  WinRow r;
+  r.lo = d.left < 0 ? 0 : p - d.left;
+  r.hi = d.right < 0 ? s.klen - 1 : min(s.klen - 1, p + d.right);
+  if (i >= s.qlen) r.hi = -1;
+  return r;
+}
+
+// LDS image of a tile: rows of DP 16-bit elements (C = DP / 8 chunks of 16 bytes), chunk c of row r at chunk c ^ f(r).  f serves both ways in which a
+// tile feeds the matrix pipe: 16 consecutive rows of one chunk (ds_read_b128) fall on 16 different chunks of 256 bytes, and the 4 rows x 64 bytes of a
+// transposed read (ds_read_b64_tr_b16) on different 64-byte groups.
+template <int DP> __device__ __forceinline__ int win_img(int row, int chunk) {
+  if constexpr (DP == 128) return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+  else if constexpr (DP == 64) return row * 128 + ((chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3))) << 4);
+  else return row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4);
+}
+
+// A operand (32 channels x 16 rows) of a tile, transposed on the way out of LDS; the 16 rows are row0 + 8 (s >> 2) + 4 (lane >> 5) + (s & 3), s = 0..7, which
+// is the order in which an accumulator's registers hold them: the exponentiated scores are the B operand as they are.
+template <int DP> __device__ __forceinline__ s16x8 win_read_tr(const unsigned char* img, int row0, int dt, int l) {
+  const int g1 = (l >> 4) & 1, qq = (l >> 2) & 3, pp = l & 3, h2 = l >> 5;
+  const int chunk = 4 * dt + 2 * g1 + (pp >> 1), sub = (pp & 1) << 3;
+  const s16x4 a = lds_read_tr16(img + win_img<DP>(row0 + 4 * h2 + qq, chunk) + sub);
+  const s16x4 b = lds_read_tr16(img + win_img<DP>(row0 + 8 + 4 * h2 + qq, chunk) + sub);
+  return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+// row of register i of a 32 x 32 accumulator
+__device__ __forceinline__ int win_acc_row(int i, int l) { return (i & 3) + 8 * (i >> 2) + 4 * (l >> 5); }
+
+// x of this lane and of lane l ^ 32
+__device__ __forceinline__ void win_halves(float x, float& u, float& v) {
+  typedef unsigned u32x2v __attribute__((ext_vector_type(2)));
+  const unsigned a = __builtin_bit_cast(unsigned, x);
+  const u32x2v sw = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  unsigned lo = sw[0], hi = sw[1];
+  asm volatile("" : "+v"(lo), "+v"(hi));  // (kept apart: hipcc folds an operation on the two results of one swap)
+  u = __builtin_bit_cast(float, lo);
+  v = __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float win_halves_max(float x) { float u, v; win_halves(x, u, v); return fmaxf(u, v); }
+__device__ __forceinline__ float win_halves_sum(float x) { float u, v; win_halves(x, u, v); return u + v; }
+
+int window_attention_check(const WinDesc& d, bool backward, const char* what);
+size_t window_attention_fwd_workspace_bytes(const WinDesc& d);
+int window_attention_fwd(const WinDesc& d, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
+size_t window_attention_bwd_workspace_bytes(const WinDesc& d, int dtype);
+int window_attention_bwd(const WinDesc& d, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
+}  // namespace smbv

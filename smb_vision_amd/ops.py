@@ -309,6 +309,307 @@ def colsum_bf16(X):
     return out
 
 
+# ---- operators of a transformer block over long token sequences: windowed attention with sinks, rotary positions with several axes, gated norms ------------
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+_EL16 = {torch.bfloat16: 0, torch.float16: 1}
+_EL = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _same_device(first, *ts):
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+
+
+def _ll3(t):
+    """Strides of the first three dimensions (a dimension of one element has no stride to speak of)."""
+    return _lib.c_ll3(*(0 if t.shape[i] <= 1 else t.stride(i) for i in range(3)))
+
+
+def _heads4(t, name, shape, dtype):
+    if t.dim() != 4 or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError(f"{name}: the channels must be contiguous")
+
+
+def _extent(t):
+    if t.numel() == 0:
+        return 0, 0
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _writable(t, name, inputs=()):
+    """An output's elements lie apart from each other and from every input."""
+    span = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
+        if s < span:
+            raise ValueError(f"{name}: elements of an output must not share memory")
+        span = (n - 1) * s + span
+    lo, hi = _extent(t)
+    for x in inputs:
+        if x is not None:
+            a, b = _extent(x)
+            if a < hi and lo < b:
+                raise ValueError(f"{name}: an output must not overlap an operand")
+
+
+def _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens):
+    _need_gpu(q, k, v, q_lens, k_lens)
+    _same_device(q, k, v, q_lens, k_lens)
+    if q.dtype not in _EL16:
+        raise ValueError(f"window attention: bf16 or fp16, got {q.dtype}")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"window attention: q [B, Sq, H, D] and k, v [B, Sk, Hk, D], got {tuple(q.shape)}, {tuple(k.shape)}")
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    _heads4(q, "q", (B, Sq, H, D), q.dtype)
+    _heads4(k, "k", (B, Sk, Hk, D), q.dtype)
+    _heads4(v, "v", (B, Sk, Hk, D), q.dtype)
+    for name, t in (("q_lens", q_lens), ("k_lens", k_lens)):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+            raise ValueError(f"{name}: a contiguous int32 tensor of {B} lengths")
+    a = _lib.WindowAttn()
+    a.dtype, a.B, a.Sq, a.Sk, a.H, a.Hk, a.Dh = _EL16[q.dtype], B, Sq, Sk, H, Hk, D
+    a.left, a.right = (min(max(int(x), -1), 2 ** 31 - 1) for x in (left, right))
+    if not 0 <= int(sinks) < 2 ** 31:
+        raise ValueError(f"sinks: {sinks}")
+    a.sinks, a.scale = int(sinks), float(D ** -0.5 if scale is None else scale)
+    a.q_lens, a.k_lens, a.q, a.k, a.v = _p(q_lens), _p(k_lens), _p(q), _p(k), _p(v)
+    a.sq, a.sk, a.sv = _ll3(q), _ll3(k), _ll3(v)
+    return a
+
+
+def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_lens=None, k_lens=None, resid=False, out=None):
+    """Softmax attention inside a sliding window, with a few first tokens that stay visible (smbv_window_attention_fwd).
+
+    q [B, Sq, H, D], k / v [B, Sk, Hk, D] (bf16 or fp16, any batch / row / head strides that are multiples of 8 elements, H a multiple of Hk, D a multiple of 8
+    up to 128).  Query i stands at position p = i + k_len - q_len and sees key j iff j < k_len, j <= p + right (right < 0: no bound; 0: causal) and
+    (j >= p - left (left < 0: no bound) or j < sinks).  q_lens / k_lens: int32 [B] on the device (None: Sq / Sk), so the queries are the last rows of their
+    sequence: all of them in training, the newest tokens against a cache in serving (Sq = 1).  A row that sees nothing, padded rows included, is 0 with lse -inf.
+    Keys that no row of a call can see are never read; a NaN or infinity in a value that SOME rows see can reach other rows near them.
+
+    Returns (o [B, Sq, H, D], lse fp32 [B, H, Sq]) and with ``resid`` also the residual of o's rounding, which window_attention_bwd takes as ``o_lo``.
+    out: a tensor for o (its strides free; with ``resid`` the residual gets a tensor of the same strides)."""
+    a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
+    lib = _lib.load()
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    _need_gpu(o)
+    _same_device(q, o)
+    _heads4(o, "out", q.shape, q.dtype)
+    _writable(o, "out", (q, k, v))
+    o_lo = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device) if resid else None
+    lse = torch.empty(a.B, a.H, a.Sq, dtype=torch.float32, device=q.device)
+    a.o, a.o_lo, a.lse, a.so = _p(o), _p(o_lo), _p(lse), _ll3(o)
+    with torch.cuda.device(q.device):
+        ws = _ws(lib.smbv_window_attention_fwd_workspace_bytes(C.byref(a)), q.device)
+        check(lib.smbv_window_attention_fwd(C.byref(a), _p(ws), ws.numel(), _stream()), "smbv_window_attention_fwd")
+    return (o, lse, o_lo) if resid else (o, lse)
+
+
+def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, scale=None, q_lens=None, k_lens=None, o_lo=None, out=None):
+    """Gradients (dq, dk, dv) of window_attention_fwd (the same keyword arguments; o, lse and o_lo as it returned them; do: the gradient of o, any strides).
+    A key head's gradient is the sum over its query heads.  Every element is written; the same call gives the same bits.  out: three tensors for the
+    gradients, for instance the column blocks of one packed gradient."""
+    a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
+    lib = _lib.load()
+    _need_gpu(o, do, lse, o_lo)
+    _same_device(q, o, do, lse, o_lo)
+    for name, t in (("o", o), ("do", do), ("o_lo", o_lo)):
+        if t is not None:
+            _heads4(t, name, q.shape, q.dtype)
+    if o_lo is not None and list(_ll3(o_lo)) != list(_ll3(o)):
+        raise ValueError("o_lo: the strides of o")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Sq) or not lse.is_contiguous():
+        raise ValueError(f"lse: a contiguous fp32 tensor of shape {(a.B, a.H, a.Sq)}")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)) if out is None else out
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        _need_gpu(t)
+        _same_device(q, t)
+        _heads4(t, name, like.shape, q.dtype)
+        _writable(t, name, (q, k, v, o, do, o_lo, lse))
+    if len({t.data_ptr() for t in (dq, dk, dv) if t.numel()}) < sum(t.numel() > 0 for t in (dq, dk, dv)):
+        raise ValueError("out: three tensors")
+    a.o, a.o_lo, a.lse, a.d_o, a.dq, a.dk, a.dv = _p(o), _p(o_lo), _p(lse), _p(do), _p(dq), _p(dk), _p(dv)
+    a.so, a.sdo, a.sdq, a.sdk, a.sdv = _ll3(o), _ll3(do), _ll3(dq), _ll3(dk), _ll3(dv)
+    with torch.cuda.device(q.device):
+        ws = _ws(lib.smbv_window_attention_bwd_workspace_bytes(C.byref(a)), q.device)
+        check(lib.smbv_window_attention_bwd(C.byref(a), _p(ws), ws.numel(), _stream()), "smbv_window_attention_bwd")
+    return dq, dk, dv
+
+
+def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=False, out=None):
+    """Rotary positions with several axes on queries and keys (smbv_rope_axes).  q [B, S, H, D], k [B, S, Hk, D] or None (bf16, fp16 or fp32, any strides with
+    contiguous channels, D even up to 1024); pos: int32 or int64 positions [axes, B, S] or [axes, S]; sections: how many pairs each of up to four axes owns,
+    in order; inv_freq: fp32 [sum(sections)].  Pair p turns by pos[its axis] * inv_freq[p]; the first 2 * sum(sections) channels of a head are the pairs
+    (p, p + sum(sections)), or (2p, 2p + 1) with ``interleaved``; the rest stays.  transpose: the inverse turn - what a gradient goes through on the way back.
+    Returns (q', k'); out: tensors for them, (q, k) themselves to turn in place."""
+    _need_gpu(q, k, pos, inv_freq)
+    _same_device(q, k, pos, inv_freq)
+    if q.dtype not in _EL:
+        raise ValueError(f"rope_axes: bf16, fp16 or fp32, got {q.dtype}")
+    if q.dim() != 4:
+        raise ValueError(f"q: expected [B, S, H, D], got {tuple(q.shape)}")
+    B, S, H, D = q.shape
+    Hk = 0 if k is None else (k.shape[2] if k.dim() == 4 else -1)
+    _heads4(q, "q", (B, S, H, D), q.dtype)
+    if k is not None:
+        _heads4(k, "k", (B, S, Hk, D), q.dtype)
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) <= 0 or 2 * sum(sections) > D:
+        raise ValueError(f"sections {sections}: one to four axes that own between them 1 .. {D // 2} pairs")
+    if pos.dtype not in (torch.int32, torch.int64) or tuple(pos.shape) not in ((len(sections), B, S), (len(sections), S)):
+        raise ValueError(f"pos: int32 or int64 of shape {(len(sections), B, S)} or {(len(sections), S)}, got {pos.dtype} {tuple(pos.shape)}")
+    if inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (sum(sections),) or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq: a contiguous fp32 tensor of {sum(sections)} frequencies")
+    lib = _lib.load()
+    qo, ko = (torch.empty(q.shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)) if out is None else out
+    for name, t, like, other in (("q", qo, q, k), ("k", ko, k, q)):
+        if (t is None) != (like is None):
+            raise ValueError("out: one tensor for each of q and k")
+        if t is None:
+            continue
+        _need_gpu(t)
+        _same_device(q, t)
+        _heads4(t, f"out of {name}", like.shape, q.dtype)
+        in_place = t.data_ptr() == like.data_ptr() and list(_ll3(t)) == list(_ll3(like))
+        # (in place beside the other operand's columns of one packed projection is fine: the elements are apart)
+        _writable(t, f"out of {name}", (pos, inv_freq) if in_place else (q, k, pos, inv_freq))
+    a = _lib.RopeAxesCfg()
+    a.dtype, a.B, a.S, a.H, a.Hk, a.Dh, a.axes = _EL[q.dtype], B, S, H, Hk, D, len(sections)
+    a.section = (C.c_int * 4)(*sections)
+    a.interleaved, a.transpose, a.pos64 = int(interleaved), int(transpose), int(pos.dtype == torch.int64)
+    a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = _p(q), _p(k), _p(qo), _p(ko), _p(pos), _p(inv_freq)
+    a.sq, a.sqo = _ll3(q), _ll3(qo)
+    if k is not None:
+        a.sk, a.sko = _ll3(k), _ll3(ko)
+    a.spos = _lib.c_ll3(pos.stride(0), pos.stride(1) if pos.dim() == 3 else 0, pos.stride(-1))
+    with torch.cuda.device(q.device):
+        check(lib.smbv_rope_axes(C.byref(a), _stream()), "smbv_rope_axes")
+    return qo, ko
+
+
+def _rows2(t, name, lead, d, dtype):
+    if t.dtype != dtype or tuple(t.shape) != (*lead, d):
+        raise ValueError(f"{name}: expected {dtype} {(*lead, d)}, got {t.dtype} {tuple(t.shape)}")
+    if d > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    try:
+        r = t.view(-1, d) if t.numel() else t.reshape(0, d)
+    except RuntimeError:
+        raise ValueError(f"{name}: the leading dimensions must have one stride between rows") from None
+    return r, (r.stride(0) if r.shape[0] > 1 else d)
+
+
+def _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps):
+    _need_gpu(h, x, post_w, post_b, gate, pre_w, pre_b)
+    _same_device(h, x, post_w, post_b, gate, pre_w, pre_b)
+    if post not in _NORMS or pre not in _NORMS:
+        raise ValueError(f"norms: 'rms', 'layer' or None, got {post!r}, {pre!r}")
+    if h.dtype not in _EL or x.dtype not in (h.dtype, torch.float32):
+        raise ValueError(f"h: bf16, fp16 or fp32; x: the same or fp32; got {h.dtype}, {x.dtype}")
+    if h.dim() < 1 or h.shape[-1] == 0:
+        raise ValueError(f"h: rows of at least one element, got {tuple(h.shape)}")
+    d, lead = h.shape[-1], tuple(h.shape[:-1])
+    a = _lib.GatedNorm()
+    hr, a.ldh = _rows2(h, "h", lead, d, h.dtype)
+    xr, a.ldx = _rows2(x, "x", lead, d, x.dtype)
+    rows = hr.shape[0]
+    for name, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (d,) or not t.is_contiguous()):
+            raise ValueError(f"{name}: a contiguous fp32 tensor of {d} elements")
+    a.h_type, a.x_type, a.d, a.post, a.pre, a.eps, a.res_scale, a.rows = _EL[h.dtype], _EL[x.dtype], d, _NORMS[post], _NORMS[pre], float(eps), float(res_scale), rows
+    a.rows_per_gate = max(rows, 1)
+    if gate is not None:
+        if gate.dtype != torch.float32 or gate.dim() < 1 or gate.shape[-1] != d or not gate.is_contiguous():
+            raise ValueError(f"gate: a contiguous fp32 tensor of rows of {d}")
+        of = list(gate.shape[:-1])
+        while of and of[-1] == 1:
+            of.pop()
+        groups = gate.numel() // d
+        if (len(lead) != 1 and tuple(of) != lead[:len(of)]) or (groups == 0) != (rows == 0 and groups == 0) or (groups and rows % groups):
+            raise ValueError(f"gate {tuple(gate.shape)}: one row, or one for each of h's leading dimensions {lead}")
+        if groups:
+            a.rows_per_gate = max(rows // groups, 1)
+    a.h, a.x, a.post_w, a.post_b, a.gate, a.pre_w, a.pre_b = _p(hr), _p(xr), _p(post_w), _p(post_b), _p(gate), _p(pre_w), _p(pre_b)
+    return a, lead, d, rows
+
+
+def gated_norm_fwd(h, x, *, post="rms", post_w=None, post_b=None, gate=None, res_scale=1.0, pre="rms", pre_w=None, pre_b=None, eps=1e-6, out=None):
+    """The norm behind a block, its gate, the scaled residual sum and the norm in front of the next block (smbv_gated_norm_fwd):
+
+        x1 = res_scale * x + gate * post(h),    y = pre(x1)
+
+    h [..., d]: the block's output (bf16, fp16, fp32); x: the residual stream (h's type or fp32); post / pre: "rms", "layer" or None, their weights and biases
+    fp32 [d] or None (1 and 0); gate: fp32 [d], or one row for each of h's leading dimensions ([B, d] or [B, 1, d] for h [B, S, d]; for h [rows, d] any
+    [n, d] whose n divides the rows: one gate for rows / n consecutive rows).  y is formed from x1 before its rounding.  Rows up to 8192 wide.
+
+    Returns (x1 in x's type, y in h's type or None without ``pre``, stats fp32 [rows, 4] for gated_norm_bwd).  out: (x1, y), x1 may be x itself."""
+    a, lead, d, rows = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
+    lib = _lib.load()
+    if out is None:
+        x1 = torch.empty((*lead, d), dtype=x.dtype, device=h.device)
+        y = torch.empty((*lead, d), dtype=h.dtype, device=h.device) if pre else None
+    else:
+        x1, y = out
+        if (y is None) != (pre is None):
+            raise ValueError("out: (x1, y), y None exactly when there is no norm in front of the next block")
+        _need_gpu(x1, y)
+        _same_device(h, x1, y)
+    x1r, a.ldx1 = _rows2(x1, "x1", lead, d, x.dtype)
+    params = (h, post_w, post_b, gate, pre_w, pre_b)
+    _writable(x1, "x1", params if x1.data_ptr() == x.data_ptr() and a.ldx1 == a.ldx else (*params, x))
+    a.x1 = _p(x1r)
+    if y is not None:
+        yr, a.ldy = _rows2(y, "y", lead, d, h.dtype)
+        _writable(y, "y", (*params, x, x1))
+        a.y = _p(yr)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=h.device)
+    a.stats = _p(stats)
+    with torch.cuda.device(h.device):
+        check(lib.smbv_gated_norm_fwd(C.byref(a), _stream()), "smbv_gated_norm_fwd")
+    return x1, y, stats
+
+
+def gated_norm_bwd(dx1, dy, h, x, stats, *, post="rms", post_w=None, post_b=None, gate=None, res_scale=1.0, pre="rms", pre_w=None, pre_b=None, out=None):
+    """Gradients of gated_norm_fwd (the same keyword arguments; h, x: its inputs; stats as it returned them).  dx1: the gradient that reaches x1 from elsewhere
+    (x's type, or None), dy: that of y (h's type; None without ``pre``).  Returns a dict: "dh", "dx" and, for every parameter that was given, its fp32
+    gradient under its name ("gate", "post_w", "post_b", "pre_w", "pre_b"; None for the others).  The same call gives the same bits.  out: (dh, dx)."""
+    a, lead, d, rows = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, 0.0)
+    lib = _lib.load()
+    _need_gpu(dx1, dy, stats)
+    _same_device(h, dx1, dy, stats)
+    if (dy is None) != (pre is None) or (dx1 is None and dy is None):
+        raise ValueError("dy: given exactly when there is a norm in front of the next block; without it dx1 is needed")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 4) or not stats.is_contiguous():
+        raise ValueError(f"stats: a contiguous fp32 tensor of shape {(rows, 4)}")
+    if dx1 is not None:
+        dx1r, a.lddx1 = _rows2(dx1, "dx1", lead, d, x.dtype)
+        a.dx1 = _p(dx1r)
+    if dy is not None:
+        dyr, a.lddy = _rows2(dy, "dy", lead, d, h.dtype)
+        a.dy = _p(dyr)
+    a.stats = _p(stats)
+    dh, dx = (torch.empty((*lead, d), dtype=h.dtype, device=h.device), torch.empty((*lead, d), dtype=x.dtype, device=h.device)) if out is None else out
+    _need_gpu(dh, dx)
+    _same_device(h, dh, dx)
+    dhr, a.lddh = _rows2(dh, "dh", lead, d, h.dtype)
+    dxr, a.lddx = _rows2(dx, "dx", lead, d, x.dtype)
+    ins = (h, x, dx1, dy, stats, post_w, post_b, gate, pre_w, pre_b)
+    _writable(dh, "dh", (*ins, dx))
+    _writable(dx, "dx", ins)
+    a.dh, a.dx = _p(dhr), _p(dxr)
+    new = torch.empty_like if rows else torch.zeros_like  # (no rows: nothing is launched, the sums are empty)
+    gr = {n: None if t is None else new(t) for n, t in (("gate", gate), ("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b))}
+    a.dgate, a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_p(gr[n]) for n in ("gate", "post_w", "post_b", "pre_w", "pre_b"))
+    with torch.cuda.device(h.device):
+        ws = _ws(lib.smbv_gated_norm_bwd_workspace_bytes(C.byref(a)), h.device)
+        check(lib.smbv_gated_norm_bwd(C.byref(a), _p(ws), ws.numel(), _stream()), "smbv_gated_norm_bwd")
+    return {"dh": dh, "dx": dx, **gr}
+
+
 def device_status(clear=False) -> int:
     """smbv_device_status: 0, or SMBV_ERR_STATE (-5) once a kernel of an earlier call has recorded a fault on the current device (text: _lib.last_error())."""
     return int(_lib.load().smbv_device_status(1 if clear else 0))
