@@ -68,6 +68,17 @@ __device__ __forceinline__ WinKeys win_keys(const WinDesc& d, const WinSeq& s, i
   w.jump = lo - w.ns;
   return w;
 }
+// How a tile of the run stands to the queries [i0, i1) (those of one wave): 0 none of them sees any of it, 2 every one sees all of it, 1 in between.
+__device__ __forceinline__ int win_tile(const WinDesc& d, const WinSeq& s, const WinKeys& w, int u0, int i0, int i1) {
+  if (i1 <= i0) return 0;
+  const int p0 = i0 + s.shift, p1 = i1 - 1 + s.shift, u1 = min(u0 + 64, w.n) - 1;
+  const int first = u0 < w.ns ? u0 : u0 + w.jump, last = u1 < w.ns ? u1 : u1 + w.jump;
+  const int inner = u0 < w.ns && u1 >= w.ns ? w.ns + w.jump : first;   // the first key behind the sinks that were put in front
+  if (d.right >= 0 && first > p1 + d.right) return 0;
+  if (d.left >= 0 && first >= d.sinks && last < p0 - d.left) return 0;
+  const bool all = u0 + 64 <= w.n && (d.right < 0 || last <= p0 + d.right) && (d.left < 0 || last < d.sinks || inner >= p1 - d.left);
+  return all ? 2 : 1;
+}
 // what one query sees: keys [0, sinks) and [lo, ...) up to hi (inclusive)
 struct WinRow { int lo, hi; };
 __device__ __forceinline__ WinRow win_row(const WinDesc& d, const WinSeq& s, int i) {
@@ -99,6 +110,66 @@ template <int DP> __device__ __forceinline__ s16x8 win_read_tr(const unsigned ch
 }
 // row of register i of a 32 x 32 accumulator
 __device__ __forceinline__ int win_acc_row(int i, int l) { return (i & 3) + 8 * (i >> 2) + 4 * (l >> 5); }
+
+// ---- tiles of 64 rows, copied global -> LDS without passing registers ----------------------------------------------------------------------------------
+// The copy is issued from asm, where the compiler does not see it (it would wait for every copy in flight in front of every LDS read): the kernels wait with
+// win_arrived() - all of this wave's copies, then the workgroup - and issue the next tile's copy right behind it, into the other of two slots.
+// One wave-instruction moves 1 KiB: lane i's 16 bytes go to LDS address lds + 16 i, from a uniform base + 32-bit offset or from a 64-bit address of its own.
+__device__ __forceinline__ void win_dma_off(const void* sbase, unsigned voff, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(voff), "s"(sbase) : "memory");
+}
+__device__ __forceinline__ void win_dma_ptr(const void* p, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(p) : "memory");
+}
+__device__ __forceinline__ void win_arrived() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's copies have landed, its reads of the other slot have returned
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// a pointer that is the same in every lane, in scalar registers
+__device__ __forceinline__ const uint16_t* win_uniform(const uint16_t* p) {
+  const unsigned long long a = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)a), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32));
+  return (const uint16_t*)(((unsigned long long)hi << 32) | lo);
+}
+
+// What one wave of four copies of a tile: piece p is the rows (NP w + p) R .. + R - 1.  The image's chunk permutation is applied on the source side.  A chunk
+// past the head's width takes the last one: the other operand of its products is zero there, or their result is not stored.
+template <int DP>
+struct WinCopy {
+  static constexpr int C = DP / 8, NP = DP / 32, R = 64 / C, IMG = 64 * DP * 2;
+  int row[NP], chunk[NP];
+  __device__ __forceinline__ WinCopy(int w, int l, int D) {
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      row[p] = (w * NP + p) * R + l / C;
+      chunk[p] = min((win_img<DP>(row[p], l % C) - row[p] * DP * 2) >> 4, D / 8 - 1);
+    }
+  }
+  // byte offsets of rows that lie at a fixed distance
+  __device__ __forceinline__ void offsets(unsigned (&off)[NP], long long rs) const {
+#pragma unroll
+    for (int p = 0; p < NP; p++) off[p] = (unsigned)(row[p] * (unsigned)rs * 2 + chunk[p] * 16);
+  }
+  // tile of run indices u0 .. u0 + 63 of the keys (an index past the run takes the run's last key: it is masked)
+  __device__ __forceinline__ void keys(const uint16_t* base, long long rs, const unsigned (&off)[NP], const WinKeys& wk, int u0, unsigned lds) const {
+    if (u0 + 64 <= wk.n && (u0 >= wk.ns || u0 + 64 <= wk.ns)) {
+      const uint16_t* s = win_uniform(base + (long long)(u0 < wk.ns ? u0 : u0 + wk.jump) * rs);
+#pragma unroll
+      for (int p = 0; p < NP; p++) win_dma_off(s, off[p], lds + p * 1024);
+    } else {
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        const int u = min(u0 + row[p], wk.n - 1);
+        win_dma_ptr(base + (long long)(u < wk.ns ? u : u + wk.jump) * rs + chunk[p] * 8, lds + p * 1024);
+      }
+    }
+  }
+};
 
 // x of this lane and of lane l ^ 32
 __device__ __forceinline__ void win_halves(float x, float& u, float& v) {

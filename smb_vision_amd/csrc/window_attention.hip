@@ -12,23 +12,13 @@
 
 namespace smbv {
 
-template <int DP>
-__device__ __forceinline__ void win_stage(unsigned char* img, const uint16_t* base, long long rs, int D, const WinKeys& wk, int u0, int t) {
-  constexpr int C = DP / 8;
-#pragma unroll
-  for (int i = 0; i < 64 * C / 256; i++) {
-    const int idx = t + 256 * i, row = idx / C, chunk = idx % C, u = u0 + row;
-    u32x4 x = {0, 0, 0, 0};
-    if (u < wk.n && chunk * 8 < D) x = *(const u32x4*)(base + (long long)(u < wk.ns ? u : u + wk.jump) * rs + chunk * 8);
-    *(u32x4*)(img + win_img<DP>(row, chunk)) = x;
-  }
-}
+static constexpr float WIN_THR = 6.f;  // log2 units
 
 template <class E, int DP>
-__global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinDesc d) {
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_fwd_kernel(WinDesc d) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2;
   using v8 = typename E::v8;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * IMG];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * IMG];   // two slots of K | V
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
   int tile, hk, b;
   xcd_block_order((int)(((long long)d.Sq * d.G + 127) / 128), d.Hk, tile, hk, b);
@@ -57,51 +47,75 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(WinDesc d) {
   float m2 = -INFINITY, sum = 0.f;
   const float c = d.scale * 1.4426950408889634f;
   const int nt = (wk.n + 63) / 64;
-  for (int j = 0; j < nt; j++) {
-    __syncthreads();
-    win_stage<DP>(smem, kb, d.sk.r, d.D, wk, 64 * j, t);
-    win_stage<DP>(smem + IMG, vb, d.sv.r, d.D, wk, 64 * j, t);
-    __syncthreads();
+  const int wi0 = win_div(d, r0 + 32 * w), wi1 = min(seq.qlen, win_div(d, min(r0 + 32 * w + 31, rows - 1)) + 1);   // this wave's queries
+  const WinCopy<DP> copy(w, l, d.D);
+  unsigned koff[WinCopy<DP>::NP], voff[WinCopy<DP>::NP];
+  copy.offsets(koff, d.sk.r);
+  copy.offsets(voff, d.sv.r);
+  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * (IMG / 4)));
+  auto stage = [&](int j, int slot) __attribute__((always_inline)) {
+    copy.keys(kb, d.sk.r, koff, wk, 64 * j, lds + slot * 2 * IMG);
+    copy.keys(vb, d.sv.r, voff, wk, 64 * j, lds + slot * 2 * IMG + IMG);
+  };
+  auto keys = [&](int j, const unsigned char* img) __attribute__((always_inline)) {
+    const int kind = win_tile(d, seq, wk, 64 * j, wi0, wi1);
+    if (kind == 0) return;
     f32x16 sc[2];
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
 #pragma unroll
       for (int x = 0; x < 16; x++) sc[kt][x] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) sc[kt] = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(smem + win_img<DP>(32 * kt + r31, 2 * ks + h2))), qf[ks], sc[kt]);
+      for (int ks = 0; ks < KS; ks++) sc[kt] = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(img + win_img<DP>(32 * kt + r31, 2 * ks + h2))), qf[ks], sc[kt]);
     }
-    float mx = -INFINITY;
+    if (kind == 1) {
 #pragma unroll
-    for (int kt = 0; kt < 2; kt++)
+      for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-      for (int x = 0; x < 16; x++) {
-        const int u = 64 * j + 32 * kt + win_acc_row(x, l), key = u < wk.ns ? u : u + wk.jump;
-        const bool vis = u < wk.n && key <= wr.hi && (key >= wr.lo || key < d.sinks);
-        sc[kt][x] = vis ? sc[kt][x] * c : -INFINITY;
-        mx = fmaxf(mx, sc[kt][x]);
-      }
-    mx = win_halves_max(mx);
-    const float m_new = fmaxf(m2, mx);
-    const float ref = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = fast_exp2(m2 - ref);
-    m2 = m_new;
-    sum *= alpha;
+        for (int x = 0; x < 16; x++) {
+          const int u = 64 * j + 32 * kt + win_acc_row(x, l), key = u < wk.ns ? u : u + wk.jump;
+          const bool vis = u < wk.n && key <= wr.hi && (key >= wr.lo || key < d.sinks);
+          sc[kt][x] = vis ? sc[kt][x] : -INFINITY;
+        }
+    }
+    float mx = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++)
+    for (int x = 1; x < 16; x++) mx = fmaxf(fmaxf(mx, sc[0][x]), sc[1][x]);
+    mx = win_halves_max(mx) * c;
+    // the running reference moves only when a score outgrows it by 2^THR: exp2 stays in range of the 16-bit P (and P keeps its relative precision)
+    if (__builtin_amdgcn_ballot_w64(mx > m2 + WIN_THR) != 0) {
+      const float m_new = fmaxf(m2, mx);
+      const float alpha = m2 == m_new ? 1.f : fast_exp2(m2 - m_new);   // (m2 = -inf: nothing is accumulated yet)
+      m2 = m_new;
+      sum *= alpha;
 #pragma unroll
-      for (int x = 0; x < 16; x++) ot[dt][x] *= alpha;
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int x = 0; x < 16; x++) ot[dt][x] *= alpha;
+    }
+    const float ref = m2 == -INFINITY ? 0.f : m2;
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
       v8 pf;
 #pragma unroll
       for (int x = 0; x < 8; x++) {
-        const float p = fast_exp2(sc[ks >> 1][8 * (ks & 1) + x] - ref);
+        const float p = fast_exp2(__builtin_fmaf(sc[ks >> 1][8 * (ks & 1) + x], c, -ref));
         sum += p;
         pf[x] = (typename E::e)p;
       }
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++) ot[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(smem + IMG, 16 * ks, dt, l)), pf, ot[dt]);
+      for (int dt = 0; dt < DT; dt++) ot[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(img + IMG, 16 * ks, dt, l)), pf, ot[dt]);
     }
+  };
+  if (nt > 0) stage(0, 0);
+  for (int j = 0; j < nt; j += 2) {
+    win_arrived();
+    if (j + 1 < nt) stage(j + 1, 1);
+    keys(j, smem);
+    if (j + 1 >= nt) break;
+    win_arrived();
+    if (j + 2 < nt) stage(j + 2, 0);
+    keys(j + 1, smem + 2 * IMG);
   }
   sum = win_halves_sum(sum);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -144,6 +158,7 @@ int window_attention_check(const WinDesc& d, bool backward, const char* what) {
       continue;
     }
     if (((uintptr_t)x.p & (x.align - 1)) || ((x.s->b | x.s->r | x.s->h) & 7)) { set_error("%s: %s must be 16-byte aligned with strides that are multiples of 8 elements", what, x.name); return SMBV_ERR_ALIGN; }
+    if (x.s->r >= (1 << 24) || x.s->h >= (1 << 24)) { set_error("%s: %s has rows or heads 2^24 elements apart", what, x.name); return SMBV_ERR_SHAPE; }   // (offsets inside a tile are 32-bit)
     if (x.s->b < 0 || x.s->r < 0 || x.s->h < 0) { set_error("%s: %s has a negative stride", what, x.name); return SMBV_ERR_SHAPE; }
   }
   if (!d.lse && d.B > 0 && d.Sq > 0) { set_error("%s: lse is null", what); return SMBV_ERR_ARG; }

@@ -44,23 +44,11 @@ __global__ __launch_bounds__(256) void win_delta_kernel(WinDesc d, int* __restri
   }
 }
 
-template <int DP>
-__device__ __forceinline__ void win_stage_keys(unsigned char* img, const uint16_t* base, long long rs, int D, const WinKeys& wk, int u0, int t) {
-  constexpr int C = DP / 8;
-#pragma unroll
-  for (int i = 0; i < 64 * C / 256; i++) {
-    const int idx = t + 256 * i, row = idx / C, chunk = idx % C, u = u0 + row;
-    u32x4 x = {0, 0, 0, 0};
-    if (u < wk.n && chunk * 8 < D) x = *(const u32x4*)(base + (long long)(u < wk.ns ? u : u + wk.jump) * rs + chunk * 8);
-    *(u32x4*)(img + win_img<DP>(row, chunk)) = x;
-  }
-}
-
 template <class E, int DP>
-__global__ __launch_bounds__(256, 1) void win_dq_kernel(WinDesc d, const int* __restrict__ expo) {
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_dq_kernel(WinDesc d, const int* __restrict__ expo) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2;
   using v8 = typename E::v8;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * IMG];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * IMG];   // two slots of K | V
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
   int tile, hk, b;
   xcd_block_order((int)(((long long)d.Sq * d.G + 127) / 128), d.Hk, tile, hk, b);
@@ -104,40 +92,65 @@ __global__ __launch_bounds__(256, 1) void win_dq_kernel(WinDesc d, const int* __
       for (int k = 0; k < 8; k++) gf[ks][k] = (_Float16)ldexpf((float)gf[ks][k], -e);
     }
   }
-  f32x16 acc[DT];
+  f32x16 acc[DT], cdel;   // cdel: -delta, the start of every dP product
 #pragma unroll
-  for (int dt = 0; dt < DT; dt++)
+  for (int x = 0; x < 16; x++) {
 #pragma unroll
-    for (int x = 0; x < 16; x++) acc[dt][x] = 0.f;
+    for (int dt = 0; dt < DT; dt++) acc[dt][x] = 0.f;
+    cdel[x] = -delta;
+  }
   const int nt = (wk.n + 63) / 64;
-  for (int j = 0; j < nt; j++) {
-    __syncthreads();
-    win_stage_keys<DP>(smem, kb, d.sk.r, d.D, wk, 64 * j, t);
-    win_stage_keys<DP>(smem + IMG, vb, d.sv.r, d.D, wk, 64 * j, t);
-    __syncthreads();
+  const int wi0 = win_div(d, r0 + 32 * w), wi1 = min(seq.qlen, win_div(d, min(r0 + 32 * w + 31, rows - 1)) + 1);   // this wave's queries
+  const WinCopy<DP> copy(w, l, d.D);
+  unsigned koff[WinCopy<DP>::NP], voff[WinCopy<DP>::NP];
+  copy.offsets(koff, d.sk.r);
+  copy.offsets(voff, d.sv.r);
+  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * (IMG / 4)));
+  auto stage = [&](int j, int slot) __attribute__((always_inline)) {
+    copy.keys(kb, d.sk.r, koff, wk, 64 * j, lds + slot * 2 * IMG);
+    copy.keys(vb, d.sv.r, voff, wk, 64 * j, lds + slot * 2 * IMG + IMG);
+  };
+  auto keys = [&](int j, const unsigned char* img) __attribute__((always_inline)) {
+    const int kind = win_tile(d, seq, wk, 64 * j, wi0, wi1);
+    if (kind == 0) return;
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
       f32x16 s, dp;
 #pragma unroll
-      for (int x = 0; x < 16; x++) { s[x] = 0.f; dp[x] = 0.f; }
+      for (int x = 0; x < 16; x++) s[x] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        s = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(smem + win_img<DP>(32 * kt + r31, 2 * ks + h2))), qf[ks], s);
-        dp = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(smem + IMG + win_img<DP>(32 * kt + r31, 2 * ks + h2))), gf[ks], dp);
+        s = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(img + win_img<DP>(32 * kt + r31, 2 * ks + h2))), qf[ks], s);
+        dp = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(img + IMG + win_img<DP>(32 * kt + r31, 2 * ks + h2))), gf[ks], ks == 0 ? cdel : dp);
+      }
+      if (kind == 1) {
+#pragma unroll
+        for (int x = 0; x < 16; x++) {
+          const int u = 64 * j + 32 * kt + win_acc_row(x, l), key = u < wk.ns ? u : u + wk.jump;
+          const bool vis = u < wk.n && key <= wr.hi && (key >= wr.lo || key < d.sinks);
+          s[x] = vis ? s[x] : -INFINITY;
+          dp[x] = vis ? dp[x] : 0.f;
+        }
       }
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         v8 ds;
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const int a = 8 * half + x, u = 64 * j + 32 * kt + win_acc_row(a, l), key = u < wk.ns ? u : u + wk.jump;
-          const bool vis = u < wk.n && key <= wr.hi && (key >= wr.lo || key < d.sinks);
-          ds[x] = (typename E::e)(vis ? fast_exp2(__builtin_fmaf(s[a], c, -lse2)) * (dp[a] - delta) : 0.f);
-        }
+        for (int x = 0; x < 8; x++) ds[x] = (typename E::e)(fast_exp2(__builtin_fmaf(s[8 * half + x], c, -lse2)) * dp[8 * half + x]);
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) acc[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(smem, 32 * kt + 16 * half, dt, l)), ds, acc[dt]);
+        for (int dt = 0; dt < DT; dt++) acc[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(img, 32 * kt + 16 * half, dt, l)), ds, acc[dt]);
       }
     }
+  };
+  if (nt > 0) stage(0, 0);
+  for (int j = 0; j < nt; j += 2) {
+    win_arrived();
+    if (j + 1 < nt) stage(j + 1, 1);
+    keys(j, smem);
+    if (j + 1 >= nt) break;
+    win_arrived();
+    if (j + 2 < nt) stage(j + 2, 0);
+    keys(j + 1, smem + 2 * IMG);
   }
   if (r >= rows) return;
   uint16_t* out = d.dq + b * d.sdq.b + i * d.sdq.r + head * d.sdq.h;
@@ -162,18 +175,37 @@ __device__ __forceinline__ void win_key_rows(const WinDesc& d, const WinSeq& s, 
   hi = ihi * d.G;
 }
 
+// rows q0 .. q0 + 63 of a key head's queries and their gradients (rows past rhi take row rhi - 1: their LSE is set to +inf).  A tile starts at a whole query
+// when 64 is a multiple of G, and its rows then lie at fixed distances.
+template <int DP>
+__device__ __forceinline__ void win_copy_rows(const WinCopy<DP>& c, const WinDesc& d, const uint16_t* base, const WinStride& st, const unsigned (&off)[WinCopy<DP>::NP],
+                                              int q0, int rhi, bool fixed, unsigned lds) {
+  if (fixed && q0 + 64 <= rhi) {
+    const uint16_t* s = win_uniform(base + (long long)win_div(d, q0) * st.r);
+#pragma unroll
+    for (int p = 0; p < WinCopy<DP>::NP; p++) win_dma_off(s, off[p], lds + p * 1024);
+  } else {
+#pragma unroll
+    for (int p = 0; p < WinCopy<DP>::NP; p++) {
+      const int r = min(q0 + c.row[p], rhi - 1), i = win_div(d, r);
+      win_dma_ptr(base + (long long)i * st.r + (long long)(r - i * d.G) * st.h + c.chunk[p] * 8, lds + p * 1024);
+    }
+  }
+}
+
+struct WinRowStat { float lse, delta; int expo; };
+
 template <class E, int DP>
-__global__ __launch_bounds__(256, 1) void win_dkv_kernel(WinDesc d, const int* __restrict__ expo) {
-  constexpr int KS = DP / 16, DT = DP / 32, C = DP / 8, IMG = 64 * DP * 2;
+__global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinDesc d, const int* __restrict__ expo) {
+  constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2;
   using v8 = typename E::v8;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * IMG];
-  __shared__ __attribute__((aligned(16))) float st_lse[64], st_delta[64];
-  __shared__ int st_lo[64], st_hi[64], st_exp[64];
+  constexpr int STAT = 64 * 5 * 4;   // LSE | delta | lo | hi | exponent of a tile's rows
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * IMG + 2 * STAT];   // two slots of Q | dO, two of the rows' numbers
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
   int tile, hk, b;
   xcd_block_order((d.Sk + 127) / 128, d.Hk, tile, hk, b);
   const WinSeq seq = win_seq(d, b);
-  const int k0 = tile * 128, key = k0 + 32 * w + r31;
+  const int k0 = tile * 128, kw0 = k0 + 32 * w, key = kw0 + r31;
   int rlo, rhi;
   win_key_rows(d, seq, k0, k0 + 128, rlo, rhi);
   const float c = d.scale * 1.4426950408889634f;
@@ -195,38 +227,54 @@ __global__ __launch_bounds__(256, 1) void win_dkv_kernel(WinDesc d, const int* _
 #pragma unroll
     for (int x = 0; x < 16; x++) { dk[dt][x] = 0.f; dv[dt][x] = 0.f; }
   int emax = WIN_NO_EXP;
-  for (int q0 = rlo; q0 < rhi; q0 += 64) {
-    __syncthreads();
+  const WinCopy<DP> copy(w, l, d.D);
+  unsigned qoff[WinCopy<DP>::NP], goff[WinCopy<DP>::NP];
 #pragma unroll
-    for (int it = 0; it < 64 * C / 256; it++) {
-      const int idx = t + 256 * it, row = idx / C, chunk = idx % C, r = q0 + row;
-      u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-      if (r < rhi && chunk * 8 < d.D) {
-        const int i = win_div(d, r), head = hk * d.G + (r - i * d.G);
-        x = *(const u32x4*)(d.q + b * d.sq.b + i * d.sq.r + head * d.sq.h + chunk * 8);
-        y = *(const u32x4*)(d.g + b * d.sg.b + i * d.sg.r + head * d.sg.h + chunk * 8);
-      }
-      *(u32x4*)(smem + win_img<DP>(row, chunk)) = x;
-      *(u32x4*)(smem + IMG + win_img<DP>(row, chunk)) = y;
+  for (int p = 0; p < WinCopy<DP>::NP; p++) {
+    const int i = win_div(d, copy.row[p]), g = copy.row[p] - i * d.G;
+    qoff[p] = (unsigned)(i * (unsigned)d.sq.r + g * (unsigned)d.sq.h) * 2 + copy.chunk[p] * 16;
+    goff[p] = (unsigned)(i * (unsigned)d.sg.r + g * (unsigned)d.sg.h) * 2 + copy.chunk[p] * 16;
+  }
+  const bool fixed = 64 % d.G == 0;
+  const uint16_t* qb = d.q + b * d.sq.b + (long long)hk * d.G * d.sq.h;
+  const uint16_t* gb = d.g + b * d.sg.b + (long long)hk * d.G * d.sg.h;
+  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * (IMG / 4)));
+  auto stage = [&](int q0, int slot) __attribute__((always_inline)) {
+    win_copy_rows<DP>(copy, d, qb, d.sq, qoff, q0, rhi, fixed, lds + slot * 2 * IMG);
+    win_copy_rows<DP>(copy, d, gb, d.sg, goff, q0, rhi, fixed, lds + slot * 2 * IMG + IMG);
+  };
+  // the first wave's lanes fetch a row's numbers a tile ahead and put them into LDS behind the products
+  auto fetch = [&](int q0) __attribute__((always_inline)) {
+    WinRowStat x = {INFINITY, 0.f, WIN_NO_EXP};
+    const int r = q0 + t;
+    if (t < 64 && r < rhi) {
+      const int i = win_div(d, r);
+      const long long at = ((long long)b * d.H + hk * d.G + (r - i * d.G)) * d.Sq + i;
+      const float ls = d.lse[at];
+      x.lse = ls == -INFINITY ? INFINITY : ls * 1.4426950408889634f;
+      x.delta = d.delta[at];
+      if constexpr (E::half) x.expo = expo[at];
     }
+    return x;
+  };
+  auto put = [&](const WinRowStat& x, int q0, int slot) __attribute__((always_inline)) {
     if (t < 64) {
-      const int r = q0 + t, i = win_div(d, r), head = hk * d.G + (r - i * d.G);
-      WinRow wr = win_row(d, seq, i);
-      float ls = INFINITY, de = 0.f;
-      int ex = WIN_NO_EXP;
-      if (r < rhi) {
-        const long long at = ((long long)b * d.H + head) * d.Sq + i;
-        const float x = d.lse[at];
-        if (x != -INFINITY) ls = x * 1.4426950408889634f;
-        de = d.delta[at];
-        if constexpr (E::half) ex = expo[at];
-      } else wr.hi = -1;
-      st_lse[t] = ls; st_delta[t] = de; st_lo[t] = wr.lo; st_hi[t] = wr.hi; st_exp[t] = ex;
+      unsigned char* at = smem + 4 * IMG + slot * STAT + 4 * t;
+      const WinRow wr = win_row(d, seq, win_div(d, q0 + t));
+      *(float*)at = x.lse;
+      *(float*)(at + 256) = -x.delta;
+      *(int*)(at + 512) = wr.lo;
+      *(int*)(at + 768) = q0 + t < rhi ? wr.hi : -1;
+      if constexpr (E::half) *(int*)(at + 1024) = x.expo;
     }
-    __syncthreads();
+  };
+  auto rowtile = [&](int q0, const unsigned char* img, const unsigned char* st) __attribute__((always_inline)) {
+    const int pa = win_div(d, q0) + seq.shift, pb = win_div(d, min(q0 + 64, rhi) - 1) + seq.shift, klast = min(kw0 + 32, seq.klen) - 1;
+    if (kw0 > klast || (d.right >= 0 && kw0 > pb + d.right) || (d.left >= 0 && kw0 >= d.sinks && klast < pa - d.left)) return;   // nobody sees these keys
+    const bool all = (d.right < 0 || klast <= pa + d.right) && (d.left < 0 || klast < d.sinks || kw0 >= pb - d.left);
     float unit = 1.f;
     if constexpr (E::half) {
-      int e = st_exp[l];
+      int e = *(const int*)(st + 1024 + 4 * l);
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 64));
       if (e > emax) {
@@ -243,34 +291,66 @@ __global__ __launch_bounds__(256, 1) void win_dkv_kernel(WinDesc d, const int* _
     for (int qt = 0; qt < 2; qt++) {
       f32x16 s, dp;
 #pragma unroll
-      for (int x = 0; x < 16; x++) { s[x] = 0.f; dp[x] = 0.f; }
+      for (int x = 0; x < 4; x++) {
+        const f32x4 de = *(const f32x4*)(st + 256 + (32 * qt + 8 * x + 4 * h2) * 4);
+#pragma unroll
+        for (int y = 0; y < 4; y++) { s[4 * x + y] = 0.f; dp[4 * x + y] = de[y]; }
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        s = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(smem + win_img<DP>(32 * qt + r31, 2 * ks + h2))), kf[ks], s);
-        dp = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(smem + IMG + win_img<DP>(32 * qt + r31, 2 * ks + h2))), vf[ks], dp);
+        s = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(img + win_img<DP>(32 * qt + r31, 2 * ks + h2))), kf[ks], s);
+        dp = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(img + IMG + win_img<DP>(32 * qt + r31, 2 * ks + h2))), vf[ks], dp);
+      }
+      if (!all) {
+#pragma unroll
+        for (int x = 0; x < 16; x++) {
+          const int row = 32 * qt + win_acc_row(x, l);
+          const bool vis = key <= *(const int*)(st + 768 + 4 * row) && (key >= *(const int*)(st + 512 + 4 * row) || key < d.sinks);
+          s[x] = vis ? s[x] : -INFINITY;
+          dp[x] = vis ? dp[x] : 0.f;
+        }
       }
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         v8 pf, ds;
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const int a = 8 * half + x, row = 32 * qt + win_acc_row(a, l);
-          const bool vis = key <= st_hi[row] && (key >= st_lo[row] || key < d.sinks);
-          const float p = vis ? fast_exp2(__builtin_fmaf(s[a], c, -st_lse[row])) : 0.f;
-          pf[x] = (typename E::e)p;
-          float g = vis ? p * (dp[a] - st_delta[row]) : 0.f;
-          if constexpr (E::half) g *= unit;
-          ds[x] = (typename E::e)g;
+        for (int x = 0; x < 2; x++) {
+          const f32x4 ls = *(const f32x4*)(st + (32 * qt + 16 * half + 8 * x + 4 * h2) * 4);
+#pragma unroll
+          for (int y = 0; y < 4; y++) {
+            const float p = fast_exp2(__builtin_fmaf(s[8 * half + 4 * x + y], c, -ls[y]));
+            pf[4 * x + y] = (typename E::e)p;
+            float g = p * dp[8 * half + 4 * x + y];
+            if constexpr (E::half) g *= unit;
+            ds[4 * x + y] = (typename E::e)g;
+          }
         }
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
-          dv[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(smem + IMG, 32 * qt + 16 * half, dt, l)), pf, dv[dt]);
-          dk[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(smem, 32 * qt + 16 * half, dt, l)), ds, dk[dt]);
+          dv[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(img + IMG, 32 * qt + 16 * half, dt, l)), pf, dv[dt]);
+          dk[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(img, 32 * qt + 16 * half, dt, l)), ds, dk[dt]);
         }
       }
     }
+  };
+  if (rlo < rhi) {
+    stage(rlo, 0);
+    put(fetch(rlo), rlo, 0);
+  }
+  for (int q0 = rlo; q0 < rhi; q0 += 128) {
+    win_arrived();
+    WinRowStat next = {INFINITY, 0.f, WIN_NO_EXP};
+    if (q0 + 64 < rhi) { stage(q0 + 64, 1); next = fetch(q0 + 64); }
+    rowtile(q0, smem, smem + 4 * IMG);
+    if (q0 + 64 >= rhi) break;
+    put(next, q0 + 64, 1);
+    win_arrived();
+    if (q0 + 128 < rhi) { stage(q0 + 128, 0); next = fetch(q0 + 128); }
+    rowtile(q0 + 64, smem + 2 * IMG, smem + 4 * IMG + STAT);
+    if (q0 + 128 < rhi) put(next, q0 + 128, 0);
   }
   if (key >= d.Sk) return;
+  const bool live = key < seq.klen;
   const float f = E::half && emax != WIN_NO_EXP ? ldexpf(d.scale, emax) : d.scale;
   uint16_t* ok = d.dk + b * d.sdk.b + key * d.sdk.r + hk * d.sdk.h;
   uint16_t* ov = d.dv + b * d.sdv.b + key * d.sdv.r + hk * d.sdv.h;
@@ -280,8 +360,11 @@ __global__ __launch_bounds__(256, 1) void win_dkv_kernel(WinDesc d, const int* _
     for (int rg = 0; rg < 4; rg++) {
       const int d0 = 32 * dt + 8 * rg + 4 * h2;
       if (d0 >= d.D) continue;
-      *(u32x2*)(ok + d0) = (u32x2){el_pack<E>(dk[dt][4 * rg] * f, dk[dt][4 * rg + 1] * f), el_pack<E>(dk[dt][4 * rg + 2] * f, dk[dt][4 * rg + 3] * f)};
-      *(u32x2*)(ov + d0) = (u32x2){el_pack<E>(dv[dt][4 * rg], dv[dt][4 * rg + 1]), el_pack<E>(dv[dt][4 * rg + 2], dv[dt][4 * rg + 3])};
+      float a[4], e[4];
+#pragma unroll
+      for (int x = 0; x < 4; x++) { a[x] = live ? dk[dt][4 * rg + x] * f : 0.f; e[x] = live ? dv[dt][4 * rg + x] : 0.f; }
+      *(u32x2*)(ok + d0) = (u32x2){el_pack<E>(a[0], a[1]), el_pack<E>(a[2], a[3])};
+      *(u32x2*)(ov + d0) = (u32x2){el_pack<E>(e[0], e[1]), el_pack<E>(e[2], e[3])};
     }
 }
 
