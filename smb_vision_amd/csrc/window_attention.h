@@ -184,7 +184,7 @@ __device__ __forceinline__ void win_halves(float x, float& u, float& v) {
 __device__ __forceinline__ float win_halves_max(float x) { float u, v; win_halves(x, u, v); return fmaxf(u, v); }
 __device__ __forceinline__ float win_halves_sum(float x) { float u, v; win_halves(x, u, v); return u + v; }
 
-int window_attention_check(const WinDesc& d, bool backward, const char* what);
+int window_attention_check(const WinDesc& d, bool backward, const char* what, bool sizes_only = false);
 size_t window_attention_fwd_workspace_bytes(const WinDesc& d);
 int window_attention_fwd(const WinDesc& d, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
 size_t window_attention_bwd_workspace_bytes(const WinDesc& d, int dtype);

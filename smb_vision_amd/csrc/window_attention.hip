@@ -141,13 +141,14 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_fwd_kernel(WinDesc
   if (h2 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !live || sum == 0.f ? -INFINITY : (m2 + __log2f(sum)) * 0.6931471805599453f;
 }
 
-int window_attention_check(const WinDesc& d, bool backward, const char* what) {
+int window_attention_check(const WinDesc& d, bool backward, const char* what, bool sizes_only) {
   if (d.B < 0 || d.Sq < 0 || d.Sk < 0 || d.Hk <= 0 || d.H <= 0 || d.H % d.Hk) { set_error("%s: bad shape B=%d Sq=%d Sk=%d H=%d Hk=%d (H a multiple of Hk)", what, d.B, d.Sq, d.Sk, d.H, d.Hk); return SMBV_ERR_SHAPE; }
   if (d.D <= 0 || d.D > 128 || (d.D & 7)) { set_error("%s: head width %d (a multiple of 8 up to 128)", what, d.D); return SMBV_ERR_SHAPE; }
   if (d.Sk >= (1 << 29) || d.Sq >= (1 << 29) || (unsigned long long)d.Sq * d.G * d.G >= (1ull << 31)) { set_error("%s: Sq=%d Sk=%d with %d heads to a key head is too long for one call", what, d.Sq, d.Sk, d.G); return SMBV_ERR_SHAPE; }
-  if (((unsigned long long)d.Sq * d.G + 63) / 64 * d.Hk * d.B >= (1ull << 30) || (unsigned long long)d.B * d.H * d.Sq >= (1ull << 40)) { set_error("%s: too many rows for one call", what); return SMBV_ERR_SHAPE; }
+  if (((unsigned long long)d.Sq * d.G + 63) / 64 * d.Hk * d.B >= (1ull << 30) || ((unsigned long long)d.Sk + 127) / 128 * d.Hk * d.B >= (1ull << 30) || (unsigned long long)d.B * d.H * d.Sq >= (1ull << 40)) { set_error("%s: too many rows for one call", what); return SMBV_ERR_SHAPE; }
   if (!(d.scale > 0.f) || !(d.scale < INFINITY)) { set_error("%s: scale must be positive and finite", what); return SMBV_ERR_ARG; }
   if (d.sinks < 0) { set_error("%s: sinks must not be negative", what); return SMBV_ERR_ARG; }
+  if (sizes_only) return SMBV_OK;
   const struct { const void* p; const WinStride* s; long long n; const char* name; bool need; int align; } t[] = {
       {d.q, &d.sq, d.Sq, "q", true, 16}, {d.k, &d.sk, d.Sk, "k", true, 16}, {d.v, &d.sv, d.Sk, "v", true, 16},
       {backward ? (const void*)d.o_in : d.o, &d.so, d.Sq, "o", true, 16}, {backward ? (const void*)d.o_lo_in : d.o_lo, &d.so, d.Sq, "o_lo", false, 16},

@@ -195,19 +195,36 @@ __device__ __forceinline__ void win_copy_rows(const WinCopy<DP>& c, const WinDes
 
 struct WinRowStat { float lse, delta; int expo; };
 
+// How the rows that see a tile of 128 keys are shared out.  The first `nsink` tiles hold sinks, which EVERY later row sees: alone they would run as long as all
+// rows are, 320 tiles of rows against 66 at 20,480 tokens and a window of 4097.  So their rows go to c1 workgroups, the other tiles' to c2 (1 unless there are too
+// few tiles to fill the chip); a tile's workgroups leave their fp32 sums in the workspace and a second launch adds them in order.
+struct WinSplit {
+  int tiles, nsink, c1, c2, units;  // units: workgroups of one key head
+  float* part;                      // [B, Hk][slots][dK | dV][128 keys][DP]
+};
+__device__ __forceinline__ int win_split_slots(const WinSplit& s) { return (s.c1 > 1 ? s.nsink * s.c1 : 0) + (s.c2 > 1 ? (s.tiles - s.nsink) * s.c2 : 0); }
+
 template <class E, int DP>
-__global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinDesc d, const int* __restrict__ expo) {
+__global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinDesc d, const int* __restrict__ expo, WinSplit sp) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2;
   using v8 = typename E::v8;
   constexpr int STAT = 64 * 5 * 4;   // LSE | delta | lo | hi | exponent of a tile's rows
   __shared__ __attribute__((aligned(16))) unsigned char smem[4 * IMG + 2 * STAT];   // two slots of Q | dO, two of the rows' numbers
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
-  int tile, hk, b;
-  xcd_block_order((d.Sk + 127) / 128, d.Hk, tile, hk, b);
+  int unit, hk, b;
+  xcd_block_order(sp.units, d.Hk, unit, hk, b);
+  const bool sink = unit < sp.nsink * sp.c1;
+  const int c12 = sink ? sp.c1 : sp.c2, rest = sink ? unit : unit - sp.nsink * sp.c1, tile = (sink ? 0 : sp.nsink) + rest / c12, share = rest % c12;
   const WinSeq seq = win_seq(d, b);
   const int k0 = tile * 128, kw0 = k0 + 32 * w, key = kw0 + r31;
   int rlo, rhi;
   win_key_rows(d, seq, k0, k0 + 128, rlo, rhi);
+  if (c12 > 1) {   // whole tiles of 64 rows to a share
+    const long long n = (rhi - rlo + 63) / 64;
+    const int lo = rlo + (int)(n * share / c12) * 64;
+    rhi = min(rhi, rlo + (int)(n * (share + 1) / c12) * 64);
+    rlo = lo;
+  }
   const float c = d.scale * 1.4426950408889634f;
   v8 kf[KS], vf[KS];
 #pragma unroll
@@ -349,9 +366,22 @@ __global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinDesc d, const int* _
     rowtile(q0 + 64, smem + 2 * IMG, smem + 4 * IMG + STAT);
     if (q0 + 128 < rhi) put(next, q0 + 128, 0);
   }
+  const float f = E::half && emax != WIN_NO_EXP ? ldexpf(d.scale, emax) : d.scale;
+  if (c12 > 1) {   // [32-channel block][key][32 channels]: a lane's four channels go out as 16 bytes
+    const int slots = win_split_slots(sp), slot = sink || sp.c1 <= 1 ? rest : sp.nsink * sp.c1 + rest;
+    float* part = sp.part + (((long long)b * d.Hk + hk) * slots + slot) * (2 * 128 * DP);
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int rg = 0; rg < 4; rg++) {
+        float* at = part + (dt * 128 + 32 * w + r31) * 32 + 8 * rg + 4 * h2;
+        *(f32x4*)at = (f32x4){dk[dt][4 * rg] * f, dk[dt][4 * rg + 1] * f, dk[dt][4 * rg + 2] * f, dk[dt][4 * rg + 3] * f};
+        *(f32x4*)(at + 128 * DP) = (f32x4){dv[dt][4 * rg], dv[dt][4 * rg + 1], dv[dt][4 * rg + 2], dv[dt][4 * rg + 3]};
+      }
+    return;
+  }
   if (key >= d.Sk) return;
   const bool live = key < seq.klen;
-  const float f = E::half && emax != WIN_NO_EXP ? ldexpf(d.scale, emax) : d.scale;
   uint16_t* ok = d.dk + b * d.sdk.b + key * d.sdk.r + hk * d.sdk.h;
   uint16_t* ov = d.dv + b * d.sdv.b + key * d.sdv.r + hk * d.sdv.h;
 #pragma unroll
@@ -368,9 +398,61 @@ __global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinDesc d, const int* _
     }
 }
 
-// workspace: delta fp32 [B, H, Sq] | exponents int32 [B, H, Sq] (fp16)
+// adds the shares of the tiles that were split: a workgroup 8 keys of one tile's dK or dV
+template <class E, int DP>
+__global__ __launch_bounds__(256) void win_dkv_join_kernel(WinDesc d, WinSplit sp) {
+  constexpr int PER = DP / 4, KEYS = 256 / PER;   // four channels a thread
+  const int split0 = sp.c1 > 1 ? 0 : sp.nsink, ntile = (sp.c2 > 1 ? sp.tiles : sp.nsink) - split0;   // the tiles [split0, split0 + ntile) were split
+  const int groups = 128 / KEYS;
+  long long x = blockIdx.x;
+  const int part = (int)(x & 1);
+  x >>= 1;
+  const int kg = (int)(x % groups);
+  x /= groups;
+  const int tile = split0 + (int)(x % ntile);
+  x /= ntile;
+  const int hk = (int)(x % d.Hk), b = (int)(x / d.Hk);
+  const bool sink = tile < sp.nsink;
+  const int c12 = sink ? sp.c1 : sp.c2, slot0 = sink ? tile * sp.c1 : (sp.c1 > 1 ? sp.nsink * sp.c1 : 0) + (tile - sp.nsink) * sp.c2;
+  const int kl = kg * KEYS + threadIdx.x / PER, ch = (threadIdx.x % PER) * 4, key = tile * 128 + kl;
+  if (key >= d.Sk || ch >= d.D) return;
+  const float* from = sp.part + (((long long)b * d.Hk + hk) * win_split_slots(sp) + slot0) * (2 * 128 * DP) + part * 128 * DP + ((ch >> 5) * 128 + kl) * 32 + (ch & 31);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < c12; i++) s += *(const f32x4*)(from + (long long)i * (2 * 128 * DP));
+  if (key >= win_seq(d, b).klen) s = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const WinStride& st = part ? d.sdv : d.sdk;
+  *(u32x2*)((part ? d.dv : d.dk) + b * st.b + key * st.r + hk * st.h + ch) = (u32x2){el_pack<E>(s[0], s[1]), el_pack<E>(s[2], s[3])};
+}
+
+static int win_dp(const WinDesc& d) { return d.D <= 32 ? 32 : d.D <= 64 ? 64 : 128; }
+static WinSplit win_split(const WinDesc& d) {
+  WinSplit s = {};
+  s.tiles = (d.Sk + 127) / 128;
+  s.nsink = d.left < 0 ? 0 : std::min(s.tiles, (int)(((long long)std::min(d.sinks, d.Sk) + 127) / 128));
+  // rows that see a tile: all (a sink, an open window to the left), or those of a window
+  const long long all = (long long)d.Sq * d.G, window = d.left < 0 || d.right < 0 ? all : std::min<long long>(all, ((long long)d.left + d.right + 128) * d.G);
+  const long long plain = (long long)(s.tiles - s.nsink) * d.Hk * d.B;
+  // A share costs its sums' way through memory (128 KiB at 128 channels, out and back) and saves a part of its tile's rows, a microsecond or two for 64 of them:
+  // no share has less than 1024 rows, and the tiles are split only as far as there is room for more workgroups (two a CU; the sinks' four)
+  s.c2 = (int)std::max<long long>(1, std::min<long long>({512 / std::max<long long>(plain, 1), window / 1024, 64}));
+  const long long share = std::max<long long>(1024, (window + s.c2 - 1) / s.c2), sinks = (long long)s.nsink * d.Hk * d.B;
+  s.c1 = (int)std::max<long long>(1, std::min<long long>({(all + share - 1) / share, 1024 / std::max<long long>(sinks, 1), 64}));
+  if (s.nsink == s.tiles) s.c2 = 1;
+  if (s.nsink == 0) s.c1 = 1;
+  s.units = s.nsink * s.c1 + (s.tiles - s.nsink) * s.c2;
+  return s;
+}
+static size_t win_split_bytes(const WinDesc& d, const WinSplit& s) {
+  const size_t slots = (size_t)(s.c1 > 1 ? s.nsink * s.c1 : 0) + (size_t)(s.c2 > 1 ? (s.tiles - s.nsink) * s.c2 : 0);
+  return slots * d.Hk * d.B * 2 * 128 * win_dp(d) * sizeof(float);
+}
+
+// workspace: delta fp32 [B, H, Sq] | exponents int32 [B, H, Sq] (fp16) | the shares of split key tiles
 static size_t win_rows_bytes(const WinDesc& d) { return ((size_t)d.B * d.H * d.Sq * 4 + 255) & ~(size_t)255; }
-size_t window_attention_bwd_workspace_bytes(const WinDesc& d, int dtype) { return win_rows_bytes(d) * (dtype ? 2 : 1) + 256; }
+size_t window_attention_bwd_workspace_bytes(const WinDesc& d, int dtype) {
+  if (window_attention_check(d, true, "window_attention_bwd", true)) return 0;
+  return win_rows_bytes(d) * (dtype ? 2 : 1) + win_split_bytes(d, win_split(d)) + 256;
+}
 
 template <class E>
 static int win_bwd(WinDesc d, void* ws, hipStream_t st) {
@@ -385,10 +467,17 @@ static int win_bwd(WinDesc d, void* ws, hipStream_t st) {
     else hipLaunchKernelGGL((win_dq_kernel<E, 128>), grid, dim3(256), 0, st, d, expo);
   }
   if (d.Sk > 0) {
-    const dim3 grid((unsigned)((d.Sk + 127) / 128 * d.Hk * d.B));
-    if (d.D <= 32) hipLaunchKernelGGL((win_dkv_kernel<E, 32>), grid, dim3(256), 0, st, d, expo);
-    else if (d.D <= 64) hipLaunchKernelGGL((win_dkv_kernel<E, 64>), grid, dim3(256), 0, st, d, expo);
-    else hipLaunchKernelGGL((win_dkv_kernel<E, 128>), grid, dim3(256), 0, st, d, expo);
+    WinSplit sp = win_split(d);
+    sp.part = (float*)((char*)ws + win_rows_bytes(d) * (E::half ? 2 : 1));
+    const dim3 grid((unsigned)((long long)sp.units * d.Hk * d.B));
+    const int ntile = (sp.c1 > 1 ? sp.nsink : 0) + (sp.c2 > 1 ? sp.tiles - sp.nsink : 0);
+#define GO(DP)                                                                                                                                    \
+  {                                                                                                                                               \
+    hipLaunchKernelGGL((win_dkv_kernel<E, DP>), grid, dim3(256), 0, st, d, expo, sp);                                                            \
+    if (ntile) hipLaunchKernelGGL((win_dkv_join_kernel<E, DP>), dim3((unsigned)(2ll * (128 / (1024 / DP)) * ntile * d.Hk * d.B)), dim3(256), 0, st, d, sp); \
+  }
+    if (d.D <= 32) GO(32) else if (d.D <= 64) GO(64) else GO(128)
+#undef GO
   }
   return check_launch("window_attention_bwd");
 }
