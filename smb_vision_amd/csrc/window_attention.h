@@ -41,7 +41,7 @@ struct WinDesc {
   const int *q_lens, *k_lens;  // per sequence; null = Sq / Sk
   const uint16_t *q, *k, *v, *o_in, *o_lo_in, *g;
   uint16_t *o, *o_lo, *dq, *dk, *dv;
-  float *lse, *delta;
+  float* lse;
   WinStride sq, sk, sv, so, sg, sdq, sdk, sdv;
 };
 
@@ -68,26 +68,20 @@ __device__ __forceinline__ WinKeys win_keys(const WinDesc& d, const WinSeq& s, i
   w.jump = lo - w.ns;
   return w;
 }
-// How a tile of the run stands to the queries [i0, i1) (those of one wave): 0 none of them sees any of it, 2 every one sees all of it, 1 in between.
-__device__ __forceinline__ int win_tile(const WinDesc& d, const WinSeq& s, const WinKeys& w, int u0, int i0, int i1) {
-  if (i1 <= i0) return 0;
-  const int p0 = i0 + s.shift, p1 = i1 - 1 + s.shift, u1 = min(u0 + 64, w.n) - 1;
-  const int first = u0 < w.ns ? u0 : u0 + w.jump, last = u1 < w.ns ? u1 : u1 + w.jump;
-  const int inner = u0 < w.ns && u1 >= w.ns ? w.ns + w.jump : first;   // the first key behind the sinks that were put in front
-  if (d.right >= 0 && first > p1 + d.right) return 0;
-  if (d.left >= 0 && first >= d.sinks && last < p0 - d.left) return 0;
-  const bool all = u0 + 64 <= w.n && (d.right < 0 || last <= p0 + d.right) && (d.left < 0 || last < d.sinks || inner >= p1 - d.left);
-  return all ? 2 : 1;
+// What one query sees of the run: indices u with u <= b and (u >= a or u < s); both bounds only grow from query to query.
+struct WinView { int a, b, s; };
+__device__ __forceinline__ WinView win_view(const WinDesc& d, const WinSeq& q, const WinKeys& w, int i) {
+  const int p = i + q.shift, lo = d.left < 0 ? 0 : p - d.left, hi = d.right < 0 ? q.klen - 1 : min(q.klen - 1, p + d.right);
+  WinView v;
+  v.s = w.ns > 0 ? w.ns : d.sinks;   // (no sinks in front of the window: the run starts at key 0, or there are none)
+  v.a = max(w.ns, lo - w.jump);
+  v.b = hi >= w.ns + w.jump ? hi - w.jump : min(hi, w.ns - 1);
+  return v;
 }
-// what one query sees: keys [0, sinks) and [lo, ...) up to hi (inclusive)
-struct WinRow { int lo, hi; };
-__device__ __forceinline__ WinRow win_row(const WinDesc& d, const WinSeq& s, int i) {
-  const int p = i + s.shift;
-  WinRow r;
-  r.lo = d.left < 0 ? 0 : p - d.left;
-  r.hi = d.right < 0 ? s.klen - 1 : min(s.klen - 1, p + d.right);
-  if (i >= s.qlen) r.hi = -1;
-  return r;
+// How a tile of 64 stands to a wave's queries, v0 the first's view and v1 the last's: 0 none sees any of it, 2 every one sees all of it, 1 in between
+__device__ __forceinline__ int win_tile(const WinView& v0, const WinView& v1, int u0) {
+  if (u0 > v1.b || (u0 >= v0.s && u0 + 63 < v0.a)) return 0;
+  return u0 + 63 <= v0.b && (u0 >= v1.a || u0 + 63 < v0.s) ? 2 : 1;
 }
 
 // LDS image of a tile: rows of DP 16-bit elements (C = DP / 8 chunks of 16 bytes), chunk c of row r at chunk c ^ f(r).  f serves both ways in which a
@@ -99,21 +93,84 @@ template <int DP> __device__ __forceinline__ int win_img(int row, int chunk) {
   else return row * 64 + ((chunk ^ ((row >> 2) & 3)) << 4);
 }
 
-// A operand (32 channels x 16 rows) of a tile, transposed on the way out of LDS; the 16 rows are row0 + 8 (s >> 2) + 4 (lane >> 5) + (s & 3), s = 0..7, which
-// is the order in which an accumulator's registers hold them: the exponentiated scores are the B operand as they are.
-template <int DP> __device__ __forceinline__ s16x8 win_read_tr(const unsigned char* img, int row0, int dt, int l) {
-  const int g1 = (l >> 4) & 1, qq = (l >> 2) & 3, pp = l & 3, h2 = l >> 5;
-  const int chunk = 4 * dt + 2 * g1 + (pp >> 1), sub = (pp & 1) << 3;
-  const s16x4 a = lds_read_tr16(img + win_img<DP>(row0 + 4 * h2 + qq, chunk) + sub);
-  const s16x4 b = lds_read_tr16(img + win_img<DP>(row0 + 8 + 4 * h2 + qq, chunk) + sub);
-  return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+// LDS addresses of this lane's operands in a tile at address `base`; everything else - the tile's slot, the 32 or 16 rows inside it - is an immediate.
+//   row[ks]    16 bytes of row (lane & 31): the A or B operand of a product over the channels
+//   tr[dt][e]  transposed: the A operand (32 channels x 16 rows) of a product over the rows; its 16 rows are 8 e + 4 (lane >> 5) + 0..3, e = 0, 1, which is
+//              the order in which an accumulator's registers hold them: exponentiated scores are the B operand as they are
+// (f has period 16 in the row, so steps of 16 rows leave the chunk's place alone)
+template <int DP> struct WinRead {
+  static constexpr int KS = DP / 16, DT = DP / 32;
+  unsigned row[KS], tr[DT][2];
+  __device__ __forceinline__ WinRead(unsigned base, int l) {
+    const int g1 = (l >> 4) & 1, qq = (l >> 2) & 3, pp = l & 3, h2 = l >> 5;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) row[ks] = base + win_img<DP>(l & 31, 2 * ks + h2);
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) tr[dt][e] = base + win_img<DP>(8 * e + 4 * h2 + qq, 4 * dt + 2 * g1 + (pp >> 1)) + ((pp & 1) << 3);
+  }
+  __device__ __forceinline__ u32x4 rows(int ks, int off) const { return *(const __attribute__((address_space(3))) u32x4*)(row[ks] + off); }
+  __device__ __forceinline__ s16x8 cols(int dt, int off) const {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(tr[dt][0] + off));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(tr[dt][1] + off));
+    return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+  // (an LDS instruction's immediate reaches 64 KiB: a ring of 128 KiB is read from one half, then the other)
+  __device__ __forceinline__ void move(int by) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) row[ks] += by;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) { tr[dt][0] += by; tr[dt][1] += by; }
+  }
+};
+__device__ __forceinline__ void win_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }  // (no copy may outlive its workgroup)
+// Walk n tiles of a ring of NS slots of SLOT bytes: arrive(), stage(tile, slot), use(tile, offset of its slot from the reader's addresses)
+template <int NS, int SLOT, class Arrive, class Stage, class Use, class Move>
+__device__ __forceinline__ void win_walk(int n, Arrive arrive, Stage stage, Use use, Move move) {
+  constexpr int HALF = NS * SLOT <= 65536 ? NS : 65536 / SLOT;   // slots within reach of one address
+  static_assert(NS % HALF == 0 && NS / HALF <= 2, "one or two halves");
+#pragma unroll
+  for (int s = 0; s < NS - 1; s++) stage(s, s);
+  for (int j = 0; j < n; j += NS) {
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      if (j + s >= n) break;
+      arrive();
+      stage(j + s + NS - 1, (s + NS - 1) % NS);
+      use(j + s, (s % HALF) * SLOT);
+      if constexpr (HALF < NS) {
+        if (s % HALF == HALF - 1) move(s < HALF ? HALF * SLOT : -HALF * SLOT);
+      }
+    }
+  }
+  win_drain();
+}
+
+// Workgroups of one key head share its keys and queries, and an XCD (every eighth workgroup) has an L2 of its own: whole key heads go to one XCD, eight at a
+// time, and what is left of them is dealt out in eight contiguous runs.  (Contiguous runs for everything put the long sequences of a ragged batch on a few XCDs.)
+__device__ __forceinline__ void win_block_order(int nt, int Hk, int B, int& tile, int& hk, int& b) {
+  const int id = blockIdx.x, heads = Hk * B, whole = heads >> 3, xcd = id & 7, slot = id >> 3;
+  int hb;
+  if (slot < whole * nt) {
+    hb = (slot / nt) * 8 + xcd;
+    tile = slot % nt;
+  } else {
+    const int n = (heads & 7) * nt, s = slot - whole * nt, q8 = n >> 3, r8 = n & 7;
+    const int g = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + s;
+    hb = whole * 8 + g / nt;
+    tile = g % nt;
+  }
+  hk = hb % Hk;
+  b = hb / Hk;
 }
 // row of register i of a 32 x 32 accumulator
 __device__ __forceinline__ int win_acc_row(int i, int l) { return (i & 3) + 8 * (i >> 2) + 4 * (l >> 5); }
 
 // ---- tiles of 64 rows, copied global -> LDS without passing registers ----------------------------------------------------------------------------------
-// The copy is issued from asm, where the compiler does not see it (it would wait for every copy in flight in front of every LDS read): the kernels wait with
-// win_arrived() - all of this wave's copies, then the workgroup - and issue the next tile's copy right behind it, into the other of two slots.
+// The copy is issued from asm, where the compiler does not see it (it would wait for every copy in flight in front of every LDS read).  A ring of NS slots: at
+// tile j the kernels wait with win_arrived() for tile j, not for the NS - 2 tiles behind it, and issue the copy of tile j + NS - 1 into the slot that tile
+// j - 1 has left.  The count is the same for every tile (one past the end copies rows that are there anyway).
 // One wave-instruction moves 1 KiB: lane i's 16 bytes go to LDS address lds + 16 i, from a uniform base + 32-bit offset or from a 64-bit address of its own.
 __device__ __forceinline__ void win_dma_off(const void* sbase, unsigned voff, unsigned lds) {
   unsigned keep;
@@ -125,8 +182,15 @@ __device__ __forceinline__ void win_dma_ptr(const void* p, unsigned lds) {
   asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "s"(lds), "v"(p) : "memory");
 }
+__device__ __forceinline__ void win_dma4_ptr(const void* p, unsigned lds) {   // 4 bytes a lane
+  unsigned keep;
+  asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(p) : "memory");
+}
+// This wave's copies have landed but for the youngest N, its reads of the slot that is filled next have returned, and so say all waves.
+template <int N>
 __device__ __forceinline__ void win_arrived() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's copies have landed, its reads of the other slot have returned
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -137,11 +201,12 @@ __device__ __forceinline__ const uint16_t* win_uniform(const uint16_t* p) {
   return (const uint16_t*)(((unsigned long long)hi << 32) | lo);
 }
 
-// What one wave of four copies of a tile: piece p is the rows (NP w + p) R .. + R - 1.  The image's chunk permutation is applied on the source side.  A chunk
+// What one of NW waves copies of a tile: piece p is the rows (NP w + p) R .. + R - 1.  The image's chunk permutation is applied on the source side.  A chunk
 // past the head's width takes the last one: the other operand of its products is zero there, or their result is not stored.
-template <int DP>
+template <int DP, int NW>
 struct WinCopy {
-  static constexpr int C = DP / 8, NP = DP / 32, R = 64 / C, IMG = 64 * DP * 2;
+  static constexpr int C = DP / 8, NP = DP / 8 / NW, R = 64 / C;
+  static_assert(NP >= 1, "a wave copies whole pieces");
   int row[NP], chunk[NP];
   __device__ __forceinline__ WinCopy(int w, int l, int D) {
 #pragma unroll

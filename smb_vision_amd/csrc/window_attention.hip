@@ -14,29 +14,40 @@ namespace smbv {
 
 static constexpr float WIN_THR = 6.f;  // log2 units
 
-template <class E, int DP>
-__global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_fwd_kernel(WinDesc d) {
-  constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2;
+// NW waves of 32 rows; NS slots of a K and a V tile
+template <class E, int DP, int NW, int NS, int OCC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void win_fwd_kernel(WinDesc d) {
+  constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BM = 32 * NW;
   using v8 = typename E::v8;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * IMG];   // two slots of K | V
+  using Copy = WinCopy<DP, NW>;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NS * 2 * IMG];
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
   int tile, hk, b;
-  xcd_block_order((int)(((long long)d.Sq * d.G + 127) / 128), d.Hk, tile, hk, b);
+  win_block_order((int)(((long long)d.Sq * d.G + BM - 1) / BM), d.Hk, d.B, tile, hk, b);
   const WinSeq seq = win_seq(d, b);
-  const int r0 = tile * 128, rows = d.Sq * d.G;
-  const int i0 = win_div(d, r0), i1 = min(seq.qlen, win_div(d, min(r0 + 127, rows - 1)) + 1);
+  const int r0 = tile * BM, rows = d.Sq * d.G;
+  const int i0 = win_div(d, r0), i1 = min(seq.qlen, win_div(d, min(r0 + BM, rows) - 1) + 1);
   const WinKeys wk = win_keys(d, seq, i0, i1);
   const int r = r0 + 32 * w + r31, i = win_div(d, r), head = hk * d.G + (r - i * d.G);
   const bool live = r < rows && i < seq.qlen;
-  WinRow wr = win_row(d, seq, i);
-  if (!live) wr.hi = -1;
+  const WinView view = win_view(d, seq, wk, i);
   const uint16_t* kb = d.k + b * d.sk.b + hk * d.sk.h;
   const uint16_t* vb = d.v + b * d.sv.b + hk * d.sv.h;
+  const Copy copy(w, l, d.D);
+  unsigned koff[Copy::NP], voff[Copy::NP];
+  copy.offsets(koff, d.sk.r);
+  copy.offsets(voff, d.sv.r);
+  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * (IMG / NW)));
+  auto stage = [&](int j, int slot) __attribute__((always_inline)) {
+    copy.keys(kb, d.sk.r, koff, wk, 64 * j, lds + slot * 2 * IMG);
+    copy.keys(vb, d.sv.r, voff, wk, 64 * j, lds + slot * 2 * IMG + IMG);
+  };
   v8 qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) {
     u32x4 x = {0, 0, 0, 0};
     if (live && 16 * ks + 8 * h2 < d.D) x = *(const u32x4*)(d.q + b * d.sq.b + i * d.sq.r + head * d.sq.h + 16 * ks + 8 * h2);
+    asm volatile("" : "+v"(x));   // (waited for here, not in the loop)
     qf[ks] = __builtin_bit_cast(v8, x);
   }
   f32x16 ot[DT];
@@ -47,18 +58,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_fwd_kernel(WinDesc
   float m2 = -INFINITY, sum = 0.f;
   const float c = d.scale * 1.4426950408889634f;
   const int nt = (wk.n + 63) / 64;
-  const int wi0 = win_div(d, r0 + 32 * w), wi1 = min(seq.qlen, win_div(d, min(r0 + 32 * w + 31, rows - 1)) + 1);   // this wave's queries
-  const WinCopy<DP> copy(w, l, d.D);
-  unsigned koff[WinCopy<DP>::NP], voff[WinCopy<DP>::NP];
-  copy.offsets(koff, d.sk.r);
-  copy.offsets(voff, d.sv.r);
-  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * (IMG / 4)));
-  auto stage = [&](int j, int slot) __attribute__((always_inline)) {
-    copy.keys(kb, d.sk.r, koff, wk, 64 * j, lds + slot * 2 * IMG);
-    copy.keys(vb, d.sv.r, voff, wk, 64 * j, lds + slot * 2 * IMG + IMG);
-  };
-  auto keys = [&](int j, const unsigned char* img) __attribute__((always_inline)) {
-    const int kind = win_tile(d, seq, wk, 64 * j, wi0, wi1);
+  // this wave's first and last query
+  const int wi0 = win_div(d, r0 + 32 * w), wi1 = min(seq.qlen, win_div(d, min(r0 + 32 * w + 32, rows) - 1) + 1);
+  const WinView v0 = win_view(d, seq, wk, wi0), v1 = win_view(d, seq, wk, wi1 - 1);
+  WinRead<DP> rd(lds_addr_of(smem), l);
+  auto keys = [&](int j, int off) __attribute__((always_inline)) {
+    const int kind = wi0 < wi1 ? win_tile(v0, v1, 64 * j) : 0;
     if (kind == 0) return;
     f32x16 sc[2];
 #pragma unroll
@@ -66,16 +71,16 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_fwd_kernel(WinDesc
 #pragma unroll
       for (int x = 0; x < 16; x++) sc[kt][x] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) sc[kt] = E::mfma(__builtin_bit_cast(v8, *(const u32x4*)(img + win_img<DP>(32 * kt + r31, 2 * ks + h2))), qf[ks], sc[kt]);
+      for (int ks = 0; ks < KS; ks++) sc[kt] = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + 64 * DP * kt)), qf[ks], sc[kt]);
     }
     if (kind == 1) {
+      const int o = 64 * j + 4 * h2, va = view.a - o, vb = view.b - o, vs = view.s - o;
 #pragma unroll
       for (int kt = 0; kt < 2; kt++)
 #pragma unroll
         for (int x = 0; x < 16; x++) {
-          const int u = 64 * j + 32 * kt + win_acc_row(x, l), key = u < wk.ns ? u : u + wk.jump;
-          const bool vis = u < wk.n && key <= wr.hi && (key >= wr.lo || key < d.sinks);
-          sc[kt][x] = vis ? sc[kt][x] : -INFINITY;
+          const int u = 32 * kt + (x & 3) + 8 * (x >> 2);
+          sc[kt][x] = u <= vb && (u >= va || u < vs) ? sc[kt][x] : -INFINITY;
         }
     }
     float mx = fmaxf(sc[0][0], sc[1][0]);
@@ -104,19 +109,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 3) void win_fwd_kernel(WinDesc
         pf[x] = (typename E::e)p;
       }
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++) ot[dt] = E::mfma(__builtin_bit_cast(v8, win_read_tr<DP>(img + IMG, 16 * ks, dt, l)), pf, ot[dt]);
+      for (int dt = 0; dt < DT; dt++) ot[dt] = E::mfma(__builtin_bit_cast(v8, rd.cols(dt, off + IMG + 32 * DP * ks)), pf, ot[dt]);
     }
   };
-  if (nt > 0) stage(0, 0);
-  for (int j = 0; j < nt; j += 2) {
-    win_arrived();
-    if (j + 1 < nt) stage(j + 1, 1);
-    keys(j, smem);
-    if (j + 1 >= nt) break;
-    win_arrived();
-    if (j + 2 < nt) stage(j + 2, 0);
-    keys(j + 1, smem + 2 * IMG);
-  }
+  if (nt > 0) win_walk<NS, 2 * IMG>(nt, win_arrived<(NS - 2) * 2 * Copy::NP>, stage, keys, [&](int by) { rd.move(by); });
   sum = win_halves_sum(sum);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   if (r >= rows) return;
@@ -168,11 +164,13 @@ int window_attention_check(const WinDesc& d, bool backward, const char* what, bo
 
 template <class E>
 static int win_fwd(const WinDesc& d, hipStream_t st) {
-  const int nt = (int)(((long long)d.Sq * d.G + 127) / 128);
-  const dim3 grid(nt * d.Hk * d.B), blk(256);
-  if (d.D <= 32) hipLaunchKernelGGL((win_fwd_kernel<E, 32>), grid, blk, 0, st, d);
-  else if (d.D <= 64) hipLaunchKernelGGL((win_fwd_kernel<E, 64>), grid, blk, 0, st, d);
-  else hipLaunchKernelGGL((win_fwd_kernel<E, 128>), grid, blk, 0, st, d);
+  const long long rows = (long long)d.Sq * d.G, heads = (long long)d.Hk * d.B;
+#define GO(DP, NW, NS, OCC) hipLaunchKernelGGL((win_fwd_kernel<E, DP, NW, NS, OCC>), dim3((unsigned)((rows + 32 * NW - 1) / (32 * NW) * heads)), dim3(64 * NW), 0, st, d)
+  if (d.D <= 32) GO(32, 4, 3, 3);
+  else if (d.D <= 64) GO(64, 4, 3, 3);
+  else if ((rows + 255) / 256 * heads >= 256) GO(128, 8, 4, 2);
+  else GO(128, 4, 4, 1);
+#undef GO
   return check_launch("window_attention_fwd");
 }
 
