@@ -78,10 +78,30 @@ __device__ __forceinline__ WinView win_view(const WinDesc& d, const WinSeq& q, c
   v.b = hi >= w.ns + w.jump ? hi - w.jump : min(hi, w.ns - 1);
   return v;
 }
-// How a tile of 64 stands to a wave's queries, v0 the first's view and v1 the last's: 0 none sees any of it, 2 every one sees all of it, 1 in between
+// How a tile of 64 stands to a wave's queries, v0 the first's view and v1 the last's
+enum { WIN_NONE = -1, WIN_ALL = 0, WIN_UPPER = 1, WIN_LOWER = 2, WIN_SINKS = 4 };   // nobody sees any of it; all see all; bounds that some row needs, sinks in the tile
 __device__ __forceinline__ int win_tile(const WinView& v0, const WinView& v1, int u0) {
-  if (u0 > v1.b || (u0 >= v0.s && u0 + 63 < v0.a)) return 0;
-  return u0 + 63 <= v0.b && (u0 >= v1.a || u0 + 63 < v0.s) ? 2 : 1;
+  if (u0 > v1.b || (u0 >= v0.s && u0 + 63 < v0.a)) return WIN_NONE;
+  return (u0 + 63 > v0.b ? WIN_UPPER : 0) | (u0 < v1.a && u0 + 63 >= v0.s ? WIN_LOWER | (u0 < v0.s ? WIN_SINKS : 0) : 0);
+}
+// Masks 32 scores: accumulator row 0 of this lane is run index o (a tile's edge needs one bound, and each costs two instructions a score)
+__device__ __forceinline__ void win_mask(f32x16& s, int kind, const WinView& v, int o) {
+  if (kind & WIN_UPPER) {
+    const int b = v.b - o;
+#pragma unroll
+    for (int x = 0; x < 16; x++) s[x] = (x & 3) + 8 * (x >> 2) <= b ? s[x] : -INFINITY;
+  }
+  if (kind & WIN_LOWER) {
+    const int a = v.a - o;
+    if (kind & WIN_SINKS) {
+      const int n = v.s - o;
+#pragma unroll
+      for (int x = 0; x < 16; x++) s[x] = (x & 3) + 8 * (x >> 2) >= a || (x & 3) + 8 * (x >> 2) < n ? s[x] : -INFINITY;
+    } else {
+#pragma unroll
+      for (int x = 0; x < 16; x++) s[x] = (x & 3) + 8 * (x >> 2) >= a ? s[x] : -INFINITY;
+    }
+  }
 }
 
 // LDS image of a tile: rows of DP 16-bit elements (C = DP / 8 chunks of 16 bytes), chunk c of row r at chunk c ^ f(r).  f serves both ways in which a
@@ -235,6 +255,10 @@ struct WinCopy {
     }
   }
 };
+
+// Left alone the compiler puts an LDS read right in front of the product that waits for it.  Code on the two sides of this line stays there: operands are read
+// on one side and used on the other, where the next ones are read.
+#define WIN_AHEAD() __builtin_amdgcn_sched_barrier(0)
 
 // x of this lane and of lane l ^ 32
 __device__ __forceinline__ void win_halves(float x, float& u, float& v) {

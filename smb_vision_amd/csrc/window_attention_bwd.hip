@@ -60,6 +60,7 @@ __global__ __launch_bounds__(256) void win_rows_kernel(WinDesc d, WinRows wr) {
 template <class E, int DP, int NW, int NS, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void win_dq_kernel(WinDesc d, WinRows wrows) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BM = 32 * NW;
+  constexpr bool AHEAD = DP == 128;   // see the forward
   using v8 = typename E::v8;
   using Copy = WinCopy<DP, NW>;
   __shared__ __attribute__((aligned(16))) unsigned char smem[NS * 2 * IMG];
@@ -126,35 +127,47 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
   };
   WinRead<DP> rd(lds_addr_of(smem), l);
   auto keys = [&](int j, int off) __attribute__((always_inline)) {
-    const int kind = wi0 < wi1 ? win_tile(v0, v1, 64 * j) : 0;
-    if (kind == 0) return;
+    const int kind = wi0 < wi1 ? win_tile(v0, v1, 64 * j) : WIN_NONE;
+    if (kind == WIN_NONE) return;
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
       f32x16 s, dp;
 #pragma unroll
       for (int x = 0; x < 16; x++) s[x] = 0.f;
+      dp = cdel;
+      u32x4 kf[KS], vf[KS];
+      auto read = [&](int ks) __attribute__((always_inline)) {
+        kf[ks] = rd.rows(ks, off + 64 * DP * kt);
+        vf[ks] = rd.rows(ks, off + IMG + 64 * DP * kt);
+      };
+      read(0);
+      read(1);
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        s = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + 64 * DP * kt)), qf[ks], s);
-        dp = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + IMG + 64 * DP * kt)), gf[ks], ks == 0 ? cdel : dp);
-      }
-      if (kind == 1) {
-        const int o = 64 * j + 32 * kt + 4 * h2, va = view.a - o, vb = view.b - o, vs = view.s - o;
+      for (int ks = 0; ks < KS; ks += 2) {   // two 16-channel steps ahead
+        if constexpr (AHEAD) WIN_AHEAD();
+        if (ks + 2 < KS) { read(ks + 2); read(ks + 3); }
 #pragma unroll
-        for (int x = 0; x < 16; x++) {
-          const int u = (x & 3) + 8 * (x >> 2);
-          const bool vis = u <= vb && (u >= va || u < vs);
-          s[x] = vis ? s[x] : -INFINITY;
-          dp[x] = vis ? dp[x] : 0.f;
+        for (int y = ks; y < ks + 2; y++) {
+          s = E::mfma(__builtin_bit_cast(v8, kf[y]), qf[y], s);
+          dp = E::mfma(__builtin_bit_cast(v8, vf[y]), gf[y], dp);
         }
       }
+      if (kind != WIN_ALL) win_mask(s, kind, view, 64 * j + 32 * kt + 4 * h2);   // (its exp2 is 0, and dP is finite as far as dO and V are)
+      s16x8 kc[2][DT];
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) kc[0][dt] = rd.cols(dt, off + 64 * DP * kt);
+      if constexpr (AHEAD) WIN_AHEAD();
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         v8 ds;
 #pragma unroll
         for (int x = 0; x < 8; x++) ds[x] = (typename E::e)(fast_exp2(__builtin_fmaf(s[8 * half + x], c, -lse2)) * dp[8 * half + x]);
+        if (half == 0) {
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) acc[dt] = E::mfma(__builtin_bit_cast(v8, rd.cols(dt, off + 64 * DP * kt + 32 * DP * half)), ds, acc[dt]);
+          for (int dt = 0; dt < DT; dt++) kc[1][dt] = rd.cols(dt, off + 64 * DP * kt + 32 * DP);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) acc[dt] = E::mfma(__builtin_bit_cast(v8, kc[half][dt]), ds, acc[dt]);
       }
     }
   };
@@ -198,7 +211,7 @@ __device__ __host__ __forceinline__ int win_split_slots(const WinSplit& s) { ret
 template <class E, int DP, int NW, int NS, int PART>
 __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wrows, const WinSplit& sp, unsigned char* smem, int unit, int hk, int b) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BK = 32 * NW, SLOT = 2 * IMG, STAT = NS * SLOT;   // STAT: where the rows' numbers lie
-  constexpr bool HAS_V = PART & 1, HAS_K = PART & 2;
+  constexpr bool HAS_V = PART & 1, HAS_K = PART & 2, AHEAD = DP == 128;   // see the forward
   using v8 = typename E::v8;
   using Copy = WinCopy<DP, NW>;
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
@@ -313,10 +326,22 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
           for (int y = 0; y < 4; y++) dp[4 * x + y] = de[y];
         }
       }
+      u32x4 qa[KS], ga[KS];
+      auto read = [&](int ks) __attribute__((always_inline)) {
+        qa[ks] = rd.rows(ks, off + 64 * DP * qt);
+        if constexpr (HAS_K) ga[ks] = rd.rows(ks, off + IMG + 64 * DP * qt);
+      };
+      read(0);
+      read(1);
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        s = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + 64 * DP * qt)), kf[ks], s);
-        if constexpr (HAS_K) dp = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + IMG + 64 * DP * qt)), vf[ks], dp);
+      for (int ks = 0; ks < KS; ks += 2) {   // two 16-channel steps ahead
+        if constexpr (AHEAD) WIN_AHEAD();
+        if (ks + 2 < KS) { read(ks + 2); read(ks + 3); }
+#pragma unroll
+        for (int y = ks; y < ks + 2; y++) {
+          s = E::mfma(__builtin_bit_cast(v8, qa[y]), kf[y], s);
+          if constexpr (HAS_K) dp = E::mfma(__builtin_bit_cast(v8, ga[y]), vf[y], dp);
+        }
       }
       if (!all) {
         const int o = q0 + 32 * qt + 4 * h2, lo = mine.lo - o, hi = min(mine.hi, rhi) - o;
@@ -328,27 +353,37 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
           if constexpr (HAS_K) dp[x] = vis ? dp[x] : 0.f;
         }
       }
+      f32x4 ls[4];
+#pragma unroll
+      for (int x = 0; x < 4; x++) ls[x] = *(const f32x4*)(st + (32 * qt + 8 * x + 4 * h2) * 4);
+      s16x8 gc[2][DT], qc[2][DT];
+      auto cols = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+          if constexpr (HAS_V) gc[half][dt] = rd.cols(dt, off + IMG + 64 * DP * qt + 32 * DP * half);
+          if constexpr (HAS_K) qc[half][dt] = rd.cols(dt, off + 64 * DP * qt + 32 * DP * half);
+        }
+      };
+      cols(0);
+      if constexpr (AHEAD) WIN_AHEAD();
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         v8 pf, ds;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const f32x4 ls = *(const f32x4*)(st + (32 * qt + 16 * half + 8 * x + 4 * h2) * 4);
-#pragma unroll
-          for (int y = 0; y < 4; y++) {
-            const float p = fast_exp2(__builtin_fmaf(s[8 * half + 4 * x + y], c, -ls[y]));
-            if constexpr (HAS_V) pf[4 * x + y] = (typename E::e)p;
-            if constexpr (HAS_K) {
-              float g = p * dp[8 * half + 4 * x + y];
-              if constexpr (E::half) g *= unit;
-              ds[4 * x + y] = (typename E::e)g;
-            }
+        for (int x = 0; x < 8; x++) {
+          const float p = fast_exp2(__builtin_fmaf(s[8 * half + x], c, -ls[2 * half + (x >> 2)][x & 3]));
+          if constexpr (HAS_V) pf[x] = (typename E::e)p;
+          if constexpr (HAS_K) {
+            float g = p * dp[8 * half + x];
+            if constexpr (E::half) g *= unit;
+            ds[x] = (typename E::e)g;
           }
         }
+        if (half == 0) cols(1);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
-          if constexpr (HAS_V) dv[dt] = E::mfma(__builtin_bit_cast(v8, rd.cols(dt, off + IMG + 64 * DP * qt + 32 * DP * half)), pf, dv[dt]);
-          if constexpr (HAS_K) dk[dt] = E::mfma(__builtin_bit_cast(v8, rd.cols(dt, off + 64 * DP * qt + 32 * DP * half)), ds, dk[dt]);
+          if constexpr (HAS_V) dv[dt] = E::mfma(__builtin_bit_cast(v8, gc[half][dt]), pf, dv[dt]);
+          if constexpr (HAS_K) dk[dt] = E::mfma(__builtin_bit_cast(v8, qc[half][dt]), ds, dk[dt]);
         }
       }
     }
@@ -389,7 +424,7 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
 // ROLES 2 (heads wider than 64): dK and dV in 128 accumulator registers beside K and V do not leave room for two waves a SIMD; workgroups of their own do, at the
 // price of a second S (5 products instead of 4).  The longer dK workgroups of a key head come first.
 template <class E, int DP, int NW, int NS, int ROLES>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 && NW == 4 ? 1 : 2, DP == 128 && NW == 4 ? 1 : 2))) void win_dkv_kernel(WinDesc d, WinRows wrows, WinSplit sp) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void win_dkv_kernel(WinDesc d, WinRows wrows, WinSplit sp) {
   __shared__ __attribute__((aligned(16))) unsigned char smem[NS * (4 * 64 * DP + 4 * 256)];   // slots of Q | dO | LSE | delta | exponent | spare
   int unit, hk, b;
   win_block_order(sp.units * ROLES, d.Hk, d.B, unit, hk, b);
@@ -424,12 +459,11 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinDesc d, WinSplit s
   *(u32x2*)((part ? d.dv : d.dk) + b * st.b + key * st.r + hk * st.h + ch) = (u32x2){el_pack<E>(s[0], s[1]), el_pack<E>(s[2], s[3])};
 }
 
-// waves a workgroup: 8 for wide heads where that still gives every CU a workgroup (they share the tiles that are copied), else 4
-static int win_dkv_waves(const WinDesc& d) { return d.D > 64 && ((long long)d.Sk + 255) / 256 * d.Hk * d.B * 2 >= 256 ? 8 : 4; }
+static constexpr int WIN_BK = 128;   // keys a workgroup (4 waves of 32)
 static int win_dp(const WinDesc& d) { return d.D <= 32 ? 32 : d.D <= 64 ? 64 : 128; }
 static WinSplit win_split(const WinDesc& d) {
   WinSplit s = {};
-  const int bk = 32 * win_dkv_waves(d);
+  const int bk = WIN_BK;
   s.roles = d.D > 64 ? 2 : 1;
   s.tiles = (d.Sk + bk - 1) / bk;
   s.nsink = d.left < 0 ? 0 : std::min(s.tiles, (int)(((long long)std::min(d.sinks, d.Sk) + bk - 1) / bk));
@@ -447,7 +481,7 @@ static WinSplit win_split(const WinDesc& d) {
   return s;
 }
 static size_t win_split_bytes(const WinDesc& d, const WinSplit& s) {
-  return (size_t)win_split_slots(s) * d.Hk * d.B * 2 * 32 * win_dkv_waves(d) * win_dp(d) * sizeof(float);
+  return (size_t)win_split_slots(s) * d.Hk * d.B * 2 * WIN_BK * win_dp(d) * sizeof(float);
 }
 
 // workspace: the rows' LSE and -delta fp32 [B, Hk, Sq G] | exponents int32 [B, Hk, Sq G] (fp16) | the shares of split key tiles
@@ -471,8 +505,7 @@ static int win_bwd(const WinDesc& d, void* ws, hipStream_t st) {
 #define GO(DP, NW, NS, OCC) hipLaunchKernelGGL((win_dq_kernel<E, DP, NW, NS, OCC>), dim3((unsigned)((rows + 32 * NW - 1) / (32 * NW) * heads)), dim3(64 * NW), 0, st, d, wr)
     if (d.D <= 32) GO(32, 4, 3, 3);
     else if (d.D <= 64) GO(64, 4, 3, 3);
-    else if ((rows + 255) / 256 * heads >= 256) GO(128, 8, 4, 2);
-    else GO(128, 4, 4, 1);
+    else GO(128, 4, 2, 2);
 #undef GO
   }
   if (d.Sk > 0) {
@@ -487,8 +520,7 @@ static int win_bwd(const WinDesc& d, void* ws, hipStream_t st) {
   }
     if (d.D <= 32) GO(32, 4, 4, 1)
     else if (d.D <= 64) GO(64, 4, 4, 1)
-    else if (win_dkv_waves(d) == 8) GO(128, 8, 4, 2)
-    else GO(128, 4, 4, 2)
+    else GO(128, 4, 2, 2)
 #undef GO
   }
   return check_launch("window_attention_bwd");
