@@ -78,11 +78,12 @@ __device__ __forceinline__ WinView win_view(const WinDesc& d, const WinSeq& q, c
   v.b = hi >= w.ns + w.jump ? hi - w.jump : min(hi, w.ns - 1);
   return v;
 }
-// How a tile of 64 stands to a wave's queries, v0 the first's view and v1 the last's
+// How a tile of T stands to a wave's queries, v0 the first's view and v1 the last's
 enum { WIN_NONE = -1, WIN_ALL = 0, WIN_UPPER = 1, WIN_LOWER = 2, WIN_SINKS = 4 };   // nobody sees any of it; all see all; bounds that some row needs, sinks in the tile
+template <int T = 64>
 __device__ __forceinline__ int win_tile(const WinView& v0, const WinView& v1, int u0) {
-  if (u0 > v1.b || (u0 >= v0.s && u0 + 63 < v0.a)) return WIN_NONE;
-  return (u0 + 63 > v0.b ? WIN_UPPER : 0) | (u0 < v1.a && u0 + 63 >= v0.s ? WIN_LOWER | (u0 < v0.s ? WIN_SINKS : 0) : 0);
+  if (u0 > v1.b || (u0 >= v0.s && u0 + T - 1 < v0.a)) return WIN_NONE;
+  return (u0 + T - 1 > v0.b ? WIN_UPPER : 0) | (u0 < v1.a && u0 + T - 1 >= v0.s ? WIN_LOWER | (u0 < v0.s ? WIN_SINKS : 0) : 0);
 }
 // Masks 32 scores: accumulator row 0 of this lane is run index o (a tile's edge needs one bound, and each costs two instructions a score)
 __device__ __forceinline__ void win_mask(f32x16& s, int kind, const WinView& v, int o) {

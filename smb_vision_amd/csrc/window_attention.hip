@@ -14,9 +14,13 @@ namespace smbv {
 
 static constexpr float WIN_THR = 6.f;  // log2 units
 
+// A call whose row tiles do not fill the chip shares their runs of keys out as well: every share leaves its maximum (log2 units), its sum and its unnormalised O,
+// and win_join_kernel joins them in the order of the shares.
+struct WinShares { int n; float* part; };   // part: [shares][B, Hk][tiles of 32 rows][32][DP + 2]: O, maximum, sum
+
 // NW waves of 32 rows; NS slots of a K and a V tile
 template <class E, int DP, int NW, int NS, int OCC>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void win_fwd_kernel(WinDesc d) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void win_fwd_kernel(WinDesc d, WinShares sh) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BM = 32 * NW;
   // Wide heads have two waves a SIMD and registers to spare: all of a tile's K operands and the first half of V's are read before the products that take them
   // (207 -> 191 us at 4 x 4093 tokens, 16 heads of 128, window 1024; at 64 channels three waves a SIMD hide the reads as well)
@@ -26,7 +30,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
   __shared__ __attribute__((aligned(16))) unsigned char smem[NS * 2 * IMG];
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
   int tile, hk, b;
-  win_block_order((int)(((long long)d.Sq * d.G + BM - 1) / BM), d.Hk, d.B, tile, hk, b);
+  win_block_order((int)(((long long)d.Sq * d.G + BM - 1) / BM) * sh.n, d.Hk, d.B, tile, hk, b);
+  const int share = tile % sh.n;
+  tile /= sh.n;
   const WinSeq seq = win_seq(d, b);
   const int r0 = tile * BM, rows = d.Sq * d.G;
   const int i0 = win_div(d, r0), i1 = min(seq.qlen, win_div(d, min(r0 + BM, rows) - 1) + 1);
@@ -41,9 +47,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
   copy.offsets(koff, d.sk.r);
   copy.offsets(voff, d.sv.r);
   const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * (IMG / NW)));
+  const long long all = (wk.n + 63) / 64;
+  const int t0 = (int)(all * share / sh.n), nt = (int)(all * (share + 1) / sh.n) - t0;   // this share's tiles
   auto stage = [&](int j, int slot) __attribute__((always_inline)) {
-    copy.keys(kb, d.sk.r, koff, wk, 64 * j, lds + slot * 2 * IMG);
-    copy.keys(vb, d.sv.r, voff, wk, 64 * j, lds + slot * 2 * IMG + IMG);
+    copy.keys(kb, d.sk.r, koff, wk, 64 * (t0 + j), lds + slot * 2 * IMG);
+    copy.keys(vb, d.sv.r, voff, wk, 64 * (t0 + j), lds + slot * 2 * IMG + IMG);
   };
   v8 qf[KS];
 #pragma unroll
@@ -60,13 +68,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
     for (int x = 0; x < 16; x++) ot[dt][x] = 0.f;
   float m2 = -INFINITY, sum = 0.f;
   const float c = d.scale * 1.4426950408889634f;
-  const int nt = (wk.n + 63) / 64;
   // this wave's first and last query
   const int wi0 = win_div(d, r0 + 32 * w), wi1 = min(seq.qlen, win_div(d, min(r0 + 32 * w + 32, rows) - 1) + 1);
   const WinView v0 = win_view(d, seq, wk, wi0), v1 = win_view(d, seq, wk, wi1 - 1);
   WinRead<DP> rd(lds_addr_of(smem), l);
   auto keys = [&](int j, int off) __attribute__((always_inline)) {
-    const int kind = wi0 < wi1 ? win_tile(v0, v1, 64 * j) : WIN_NONE;
+    const int kind = wi0 < wi1 ? win_tile(v0, v1, 64 * (t0 + j)) : WIN_NONE;
     if (kind == WIN_NONE) return;
     f32x16 sc[2];
     u32x4 kf[2][KS];
@@ -87,7 +94,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
     }
     if (kind != WIN_ALL) {
 #pragma unroll
-      for (int kt = 0; kt < 2; kt++) win_mask(sc[kt], kind, view, 64 * j + 32 * kt + 4 * h2);
+      for (int kt = 0; kt < 2; kt++) win_mask(sc[kt], kind, view, 64 * (t0 + j) + 32 * kt + 4 * h2);
     }
     float mx = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
@@ -133,6 +140,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
   };
   if (nt > 0) win_walk<NS, 2 * IMG>(nt, win_arrived<(NS - 2) * 2 * Copy::NP>, stage, keys, [&](int by) { rd.move(by); });
   sum = win_halves_sum(sum);
+  if (sh.n > 1) {
+    const int tiles = (rows + 31) / 32;
+    if (r0 + 32 * w >= rows) return;
+    float* out = sh.part + ((((long long)share * d.B + b) * d.Hk + hk) * tiles + tile * NW + w) * (32 * (DP + 2)) + r31 * (DP + 2);
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int x = 0; x < 16; x += 2) *(float2*)(out + 32 * dt + win_acc_row(x, l)) = make_float2(ot[dt][x], ot[dt][x + 1]);   // (rows of DP + 2 floats)
+    if (h2 == 0) *(float2*)(out + DP) = make_float2(m2, sum);
+    return;
+  }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   if (r >= rows) return;
   const long long oo = b * d.so.b + i * d.so.r + head * d.so.h;
@@ -154,6 +172,198 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
       }
     }
   if (h2 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !live || sum == 0.f ? -INFINITY : (m2 + __log2f(sum)) * 0.6931471805599453f;
+}
+
+// ---- few rows against many keys (single tokens) ------------------------------------------------------------------------------------------------------------
+// Bound by HBM: every key and value is read once for a handful of rows.  A workgroup takes 32 rows of one key head and a share of their run of keys; its four
+// waves take 32-key tiles in turn, each with a ring of its own, so nobody waits for anybody until their sums are joined in LDS.  (16 single tokens on caches of
+// 16,384 keys, 8 key heads of 128, window 8192: 216 us by the 128-row kernel, one wave of which has rows; 110 us, 4.8 TB/s, here.)
+// a row's N channels from ch0 on: O normalised, its residual, and by the first of the row's threads the LSE
+template <class E, int N>
+__device__ __forceinline__ void win_few_store(const WinDesc& d, const float (&o)[N], int ch0, int rr, int hk, int b, float m, float total, const WinSeq& seq) {
+  const int i = win_div(d, rr), head = hk * d.G + (rr - i * d.G);
+  const bool live = i < seq.qlen;
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  const long long oo = b * d.so.b + i * d.so.r + head * d.so.h + ch0;
+#pragma unroll
+  for (int x = 0; x < N; x += 4) {
+    if (ch0 + x >= d.D) continue;
+    float f[4];
+#pragma unroll
+    for (int y = 0; y < 4; y++) f[y] = live ? o[x + y] * inv : 0.f;
+    const u32x2 pk = {el_pack<E>(f[0], f[1]), el_pack<E>(f[2], f[3])};
+    *(u32x2*)(d.o + oo + x) = pk;
+    if (d.o_lo) {
+#pragma unroll
+      for (int y = 0; y < 4; y++) f[y] -= el_f<E>((uint16_t)(pk[y >> 1] >> (16 * (y & 1))));
+      *(u32x2*)(d.o_lo + oo + x) = (u32x2){el_pack<E>(f[0], f[1]), el_pack<E>(f[2], f[3])};
+    }
+  }
+  if (ch0 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !live || total == 0.f ? -INFINITY : (m + __log2f(total)) * 0.6931471805599453f;
+}
+
+template <class E, int DP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 4))) void win_few_kernel(WinDesc d, WinShares sh) {
+  constexpr int KS = DP / 16, DT = DP / 32, IMG = 32 * DP * 2, NS = DP == 32 ? 3 : 2, RING = NS * 2 * IMG, NP = IMG / 1024, R = 512 / DP, C = DP / 8;
+  using v8 = typename E::v8;
+  constexpr int JOIN = 4 * 32 * (DP + 4) * 4;   // the waves' O (rows of DP + 4 floats: the 16-byte pieces of a row fall on different banks), maximum, sum
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * RING > JOIN ? 4 * RING : JOIN];
+  const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
+  const int rows = d.Sq * d.G, tiles = (rows + 31) / 32;
+  int unit, hk, b;
+  win_block_order(tiles * sh.n, d.Hk, d.B, unit, hk, b);
+  const int tile = unit / sh.n, share = unit - tile * sh.n;
+  const WinSeq seq = win_seq(d, b);
+  const int r0 = tile * 32, i0 = win_div(d, r0), i1 = min(seq.qlen, win_div(d, min(r0 + 32, rows) - 1) + 1);
+  const WinKeys wk = win_keys(d, seq, i0, i1);
+  const int r = r0 + r31, i = win_div(d, r), head = hk * d.G + (r - i * d.G);
+  const bool live = r < rows && i < seq.qlen;
+  const WinView view = win_view(d, seq, wk, i), v0 = win_view(d, seq, wk, i0), v1 = win_view(d, seq, wk, i1 - 1);
+  const uint16_t* kb = d.k + b * d.sk.b + hk * d.sk.h;
+  const uint16_t* vb = d.v + b * d.sv.b + hk * d.sv.h;
+  // this share's tiles of 32 keys [t0, t1), this wave's: t0 + w, t0 + w + 4, ...
+  const long long nt = (wk.n + 31) / 32;
+  const int t0 = (int)(nt * share / sh.n), t1 = (int)(nt * (share + 1) / sh.n), mine = t1 - t0 > w ? (t1 - t0 - w + 3) / 4 : 0;
+  const unsigned lds = __builtin_amdgcn_readfirstlane((int)(lds_addr_of(smem) + w * RING));
+  auto stage = [&](int j, int slot) __attribute__((always_inline)) {
+    const int u0 = 32 * (t0 + w + 4 * j);
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      const int row = p * R + l / C, chunk = min((win_img<DP>(row, l % C) - row * DP * 2) >> 4, d.D / 8 - 1), u = min(u0 + row, wk.n - 1);
+      const long long key = u < wk.ns ? u : u + wk.jump;
+      win_dma_ptr(kb + key * d.sk.r + chunk * 8, lds + slot * 2 * IMG + p * 1024);
+      win_dma_ptr(vb + key * d.sv.r + chunk * 8, lds + slot * 2 * IMG + IMG + p * 1024);
+    }
+  };
+  if (mine > 0) {
+#pragma unroll
+    for (int s = 0; s < NS - 1; s++) stage(s, s);
+  }
+  v8 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) {
+    u32x4 x = {0, 0, 0, 0};
+    if (live && 16 * ks + 8 * h2 < d.D) x = *(const u32x4*)(d.q + b * d.sq.b + i * d.sq.r + head * d.sq.h + 16 * ks + 8 * h2);
+    asm volatile("" : "+v"(x));
+    qf[ks] = __builtin_bit_cast(v8, x);
+  }
+  f32x16 ot[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+    for (int x = 0; x < 16; x++) ot[dt][x] = 0.f;
+  float m2 = -INFINITY, sum = 0.f;
+  const float c = d.scale * 1.4426950408889634f;
+  const WinRead<DP> rd(lds, l);
+  for (int j = 0; j < mine; j += NS) {
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      if (j + s >= mine) break;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (this wave's reads of the slot that is filled next have returned)
+      stage(j + s + NS - 1, (s + NS - 1) % NS);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * 2 * NP) : "memory");
+      const int off = s * 2 * IMG, u0 = 32 * (t0 + w + 4 * (j + s));
+      f32x16 sc;
+#pragma unroll
+      for (int x = 0; x < 16; x++) sc[x] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) sc = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off)), qf[ks], sc);
+      const int kind = win_tile<32>(v0, v1, u0);
+      if (kind != WIN_ALL) win_mask(sc, kind == WIN_NONE ? WIN_UPPER | WIN_LOWER | WIN_SINKS : kind, view, u0 + 4 * h2);
+      float mx = sc[0];
+#pragma unroll
+      for (int x = 1; x < 15; x += 2) mx = fmaxf(fmaxf(mx, sc[x]), sc[x + 1]);
+      mx = win_halves_max(fmaxf(mx, sc[15])) * c;
+      if (__builtin_amdgcn_ballot_w64(mx > m2 + WIN_THR) != 0) {
+        const float m_new = fmaxf(m2, mx), alpha = m2 == m_new ? 1.f : fast_exp2(m2 - m_new);
+        m2 = m_new;
+        sum *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int x = 0; x < 16; x++) ot[dt][x] *= alpha;
+      }
+      const float ref = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+        v8 pf;
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const float p = fast_exp2(__builtin_fmaf(sc[8 * ks + x], c, -ref));
+          sum += p;
+          pf[x] = (typename E::e)p;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) ot[dt] = E::mfma(__builtin_bit_cast(v8, rd.cols(dt, off + IMG + 32 * DP * ks)), pf, ot[dt]);
+      }
+    }
+  }
+  win_drain();
+  sum = win_halves_sum(sum);
+  __syncthreads();
+  // join the four waves: row r31's O in LDS [wave][row][DP + 4], then its maximum and sum
+  float* join = (float*)smem;
+  constexpr int LD = DP + 4;
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+    for (int rg = 0; rg < 4; rg++)
+      *(f32x4*)(join + (w * 32 + r31) * LD + 32 * dt + 8 * rg + 4 * h2) = (f32x4){ot[dt][4 * rg], ot[dt][4 * rg + 1], ot[dt][4 * rg + 2], ot[dt][4 * rg + 3]};
+  if (h2 == 0) { join[(w * 32 + r31) * LD + DP] = m2; join[(w * 32 + r31) * LD + DP + 1] = sum; }
+  __syncthreads();
+  const int row = t >> 3, ch0 = (t & 7) * (DP / 8);   // 8 threads a row
+  const float* mr = join + row * LD + DP;
+  float m = -INFINITY, wgt[4], total = 0.f;
+#pragma unroll
+  for (int x = 0; x < 4; x++) m = fmaxf(m, mr[x * 32 * LD]);
+#pragma unroll
+  for (int x = 0; x < 4; x++) {
+    wgt[x] = m == -INFINITY ? 0.f : fast_exp2(mr[x * 32 * LD] - m);
+    total += wgt[x] * mr[x * 32 * LD + 1];
+  }
+  float o[DP / 8];
+#pragma unroll
+  for (int x = 0; x < DP / 8; x += 4) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int y = 0; y < 4; y++) a += *(const f32x4*)(join + (y * 32 + row) * LD + ch0 + x) * wgt[y];
+    o[x] = a[0]; o[x + 1] = a[1]; o[x + 2] = a[2]; o[x + 3] = a[3];
+  }
+  if (sh.n > 1) {
+    float* out = sh.part + ((((long long)share * d.B + b) * d.Hk + hk) * tiles + tile) * (32 * (DP + 2)) + row * (DP + 2);
+#pragma unroll
+    for (int x = 0; x < DP / 8; x += 2) *(float2*)(out + ch0 + x) = make_float2(o[x], o[x + 1]);
+    if (ch0 == 0) { out[DP] = m; out[DP + 1] = total; }
+    return;
+  }
+  const int rr = r0 + row;
+  if (rr >= rows) return;
+  win_few_store<E, DP / 8>(d, o, ch0, rr, hk, b, m, total, seq);
+}
+
+template <class E, int DP>
+__global__ __launch_bounds__(256) void win_join_kernel(WinDesc d, WinShares sh) {
+  const int rows = d.Sq * d.G, tiles = (rows + 31) / 32;
+  const long long x = (long long)blockIdx.x * 32 + (threadIdx.x >> 3), per = (long long)rows;
+  if (x >= per * d.Hk * d.B) return;
+  const int hb = (int)(x / per), rr = (int)(x - hb * per), hk = hb % d.Hk, b = hb / d.Hk, ch0 = (threadIdx.x & 7) * (DP / 8);
+  const long long step = (long long)d.B * d.Hk * tiles * (32 * (DP + 2));
+  const float* at = sh.part + ((long long)hb * tiles + rr / 32) * (32 * (DP + 2)) + (rr % 32) * (DP + 2);
+  float m = -INFINITY, total = 0.f, o[DP / 8];
+  for (int s = 0; s < sh.n; s++) m = fmaxf(m, at[s * step + DP]);
+#pragma unroll
+  for (int i = 0; i < DP / 8; i++) o[i] = 0.f;
+  for (int s = 0; s < sh.n; s++) {
+    const float w = m == -INFINITY ? 0.f : fast_exp2(at[s * step + DP] - m);
+    total += w * at[s * step + DP + 1];
+#pragma unroll
+    for (int i = 0; i < DP / 8; i += 2) {
+      const float2 p = *(const float2*)(at + s * step + ch0 + i);
+      o[i] += w * p.x;
+      o[i + 1] += w * p.y;
+    }
+  }
+  win_few_store<E, DP / 8>(d, o, ch0, rr, hk, b, m, total, win_seq(d, b));
 }
 
 int window_attention_check(const WinDesc& d, bool backward, const char* what, bool sizes_only) {
@@ -181,22 +391,54 @@ int window_attention_check(const WinDesc& d, bool backward, const char* what, bo
   return SMBV_OK;
 }
 
-template <class E>
-static int win_fwd(const WinDesc& d, hipStream_t st) {
+// Up to 64 rows a key head go to the 32-row kernel: at 128 rows most of a workgroup would have none.  Shares: as many as bring every CU the workgroups that it
+// holds (by LDS and registers: one at 128 channels and few rows, else two or three), none with less than 256 (512) keys, which cost about what a share's sums do.
+struct WinPlan { bool few; int shares; };
+static WinPlan win_plan(const WinDesc& d) {
   const long long rows = (long long)d.Sq * d.G, heads = (long long)d.Hk * d.B;
-#define GO(DP, NW, NS, OCC) hipLaunchKernelGGL((win_fwd_kernel<E, DP, NW, NS, OCC>), dim3((unsigned)((rows + 32 * NW - 1) / (32 * NW) * heads)), dim3(64 * NW), 0, st, d)
-  if (d.D <= 32) GO(32, 4, 3, 4);
-  else if (d.D <= 64) GO(64, 4, 3, 3);
-  else GO(128, 4, 2, 2);
+  WinPlan p;
+  p.few = rows <= 64;
+  const int tile = p.few ? 32 : 128;
+  const long long units = std::max<long long>(1, (rows + tile - 1) / tile * heads), room = p.few ? (d.D > 64 ? 256 : 512) : (d.D > 64 ? 512 : 768);
+  long long keys = d.Sk;   // of a row tile at most
+  if (d.left >= 0 && d.right >= 0) keys = std::min<long long>(keys, (long long)d.left + d.right + tile + d.sinks);
+  p.shares = (int)std::max<long long>(1, std::min<long long>(room / units, keys / (p.few ? 256 : 512)));
+  return p;
+}
+static size_t win_shares_bytes(const WinDesc& d) {
+  const int dp = d.D <= 32 ? 32 : d.D <= 64 ? 64 : 128, n = win_plan(d).shares;
+  return n > 1 ? (size_t)n * d.B * d.Hk * (((size_t)d.Sq * d.G + 31) / 32) * 32 * (dp + 2) * sizeof(float) : 0;
+}
+
+template <class E>
+static int win_fwd(const WinDesc& d, void* ws, hipStream_t st) {
+  const long long rows = (long long)d.Sq * d.G, heads = (long long)d.Hk * d.B;
+  const WinPlan p = win_plan(d);
+  const WinShares sh = {p.shares, (float*)ws};
+  const dim3 few((unsigned)((rows + 31) / 32 * sh.n * heads)), many((unsigned)((rows + 127) / 128 * sh.n * heads)), join((unsigned)((rows * heads + 31) / 32));
+#define GO(DP, NS, OCC)                                                                                                     \
+  {                                                                                                                         \
+    if (p.few) hipLaunchKernelGGL((win_few_kernel<E, DP>), few, dim3(256), 0, st, d, sh);                                   \
+    else hipLaunchKernelGGL((win_fwd_kernel<E, DP, 4, NS, OCC>), many, dim3(256), 0, st, d, sh);                            \
+    if (sh.n > 1) hipLaunchKernelGGL((win_join_kernel<E, DP>), join, dim3(256), 0, st, d, sh);                              \
+  }
+  if (d.D <= 32) GO(32, 3, 4) else if (d.D <= 64) GO(64, 3, 3) else GO(128, 2, 2)
 #undef GO
   return check_launch("window_attention_fwd");
 }
 
-size_t window_attention_fwd_workspace_bytes(const WinDesc&) { return 256; }
+// workspace: the shares' sums
+size_t window_attention_fwd_workspace_bytes(const WinDesc& d) {
+  if (window_attention_check(d, false, "window_attention_fwd", true)) return 0;
+  return win_shares_bytes(d) + 256;
+}
+
 int window_attention_fwd(const WinDesc& d, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
   if (int rc = window_attention_check(d, false, "window_attention_fwd")) return rc;
   if (d.B == 0 || d.Sq == 0) return SMBV_OK;
-  return dtype == 0 ? win_fwd<ElBf16>(d, st) : win_fwd<ElF16>(d, st);
+  const size_t need = window_attention_fwd_workspace_bytes(d);
+  if (need > 256 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255))) { set_error("window_attention_fwd: workspace short or not 256-byte aligned (%zu < %zu)", ws_bytes, need); return SMBV_ERR_WORKSPACE; }
+  return dtype == 0 ? win_fwd<ElBf16>(d, ws, st) : win_fwd<ElF16>(d, ws, st);
 }
 
 }  // namespace smbv
