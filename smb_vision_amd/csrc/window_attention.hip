@@ -15,8 +15,12 @@ namespace smbv {
 static constexpr float WIN_THR = 6.f;  // log2 units
 
 // A call whose row tiles do not fill the chip shares their runs of keys out as well: every share leaves its maximum (log2 units), its sum and its unnormalised O,
-// and win_join_kernel joins them in the order of the shares.
-struct WinShares { int n; float* part; };   // part: [shares][B, Hk][tiles of 32 rows][32][DP + 2]: O, maximum, sum
+// and win_join_kernel joins them, always in the same order.
+// part: [shares][B, Hk][tiles of 32 rows], each [DP / 32][32 rows][32 channels] of O, then [32 rows] pairs of maximum and sum
+struct WinShares { int n; float* part; };
+template <int DP> __device__ __forceinline__ float* win_part(const WinDesc& d, const WinShares& sh, int share, int b, int hk, int tile32, int tiles32) {
+  return sh.part + ((((long long)share * d.B + b) * d.Hk + hk) * tiles32 + tile32) * (32 * (DP + 2));
+}
 
 // NW waves of 32 rows; NS slots of a K and a V tile
 template <class E, int DP, int NW, int NS, int OCC>
@@ -143,12 +147,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
   if (sh.n > 1) {
     const int tiles = (rows + 31) / 32;
     if (r0 + 32 * w >= rows) return;
-    float* out = sh.part + ((((long long)share * d.B + b) * d.Hk + hk) * tiles + tile * NW + w) * (32 * (DP + 2)) + r31 * (DP + 2);
+    float* out = win_part<DP>(d, sh, share, b, hk, tile * NW + w, tiles);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-      for (int x = 0; x < 16; x += 2) *(float2*)(out + 32 * dt + win_acc_row(x, l)) = make_float2(ot[dt][x], ot[dt][x + 1]);   // (rows of DP + 2 floats)
-    if (h2 == 0) *(float2*)(out + DP) = make_float2(m2, sum);
+      for (int rg = 0; rg < 4; rg++)
+        if (32 * dt + 8 * rg < d.D) *(f32x4*)(out + (dt * 32 + r31) * 32 + 8 * rg + 4 * h2) = (f32x4){ot[dt][4 * rg], ot[dt][4 * rg + 1], ot[dt][4 * rg + 2], ot[dt][4 * rg + 3]};
+    if (h2 == 0) *(float2*)(out + 32 * DP + 2 * r31) = make_float2(m2, sum);
     return;
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -330,10 +335,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 4))) voi
     o[x] = a[0]; o[x + 1] = a[1]; o[x + 2] = a[2]; o[x + 3] = a[3];
   }
   if (sh.n > 1) {
-    float* out = sh.part + ((((long long)share * d.B + b) * d.Hk + hk) * tiles + tile) * (32 * (DP + 2)) + row * (DP + 2);
+    float* out = win_part<DP>(d, sh, share, b, hk, tile, tiles);
 #pragma unroll
-    for (int x = 0; x < DP / 8; x += 2) *(float2*)(out + ch0 + x) = make_float2(o[x], o[x + 1]);
-    if (ch0 == 0) { out[DP] = m; out[DP + 1] = total; }
+    for (int x = 0; x < DP / 8; x += 4)
+      if (ch0 + x < d.D) *(f32x4*)(out + (((ch0 + x) >> 5) * 32 + row) * 32 + ((ch0 + x) & 31)) = (f32x4){o[x], o[x + 1], o[x + 2], o[x + 3]};
+    if (ch0 == 0) *(float2*)(out + 32 * DP + 2 * row) = make_float2(m, total);
     return;
   }
   const int rr = r0 + row;
@@ -341,29 +347,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 4))) voi
   win_few_store<E, DP / 8>(d, o, ch0, rr, hk, b, m, total, seq);
 }
 
-template <class E, int DP>
+// 8 lanes a row's channels, SG groups of them its shares (8 where there are many: one after the other they took 31 us for 32 shares of 64 rows)
+template <class E, int DP, int SG>
 __global__ __launch_bounds__(256) void win_join_kernel(WinDesc d, WinShares sh) {
-  const int rows = d.Sq * d.G, tiles = (rows + 31) / 32;
-  const long long x = (long long)blockIdx.x * 32 + (threadIdx.x >> 3), per = (long long)rows;
-  if (x >= per * d.Hk * d.B) return;
-  const int hb = (int)(x / per), rr = (int)(x - hb * per), hk = hb % d.Hk, b = hb / d.Hk, ch0 = (threadIdx.x & 7) * (DP / 8);
-  const long long step = (long long)d.B * d.Hk * tiles * (32 * (DP + 2));
-  const float* at = sh.part + ((long long)hb * tiles + rr / 32) * (32 * (DP + 2)) + (rr % 32) * (DP + 2);
+  const int rows = d.Sq * d.G, tiles = (rows + 31) / 32, l = threadIdx.x & (8 * SG - 1), ch0 = (l & 7) * (DP / 8);
+  const long long x = (long long)blockIdx.x * (32 / SG) + threadIdx.x / (8 * SG);
+  if (x >= (long long)rows * d.Hk * d.B) return;
+  const int hb = (int)(x / rows), rr = (int)(x - (long long)hb * rows), hk = hb % d.Hk, b = hb / d.Hk, row = rr & 31;
   float m = -INFINITY, total = 0.f, o[DP / 8];
-  for (int s = 0; s < sh.n; s++) m = fmaxf(m, at[s * step + DP]);
 #pragma unroll
   for (int i = 0; i < DP / 8; i++) o[i] = 0.f;
-  for (int s = 0; s < sh.n; s++) {
-    const float w = m == -INFINITY ? 0.f : fast_exp2(at[s * step + DP] - m);
-    total += w * at[s * step + DP + 1];
+  for (int s = l >> 3; s < sh.n; s += SG) {
+    const float* at = win_part<DP>(d, sh, s, b, hk, rr >> 5, tiles);
+    const float2 ms = *(const float2*)(at + 32 * DP + 2 * row);
+    const float mn = fmaxf(m, ms.x), keep = m == -INFINITY ? 0.f : fast_exp2(m - mn), w = ms.x == -INFINITY ? 0.f : fast_exp2(ms.x - mn);
+    m = mn;
+    total = total * keep + w * ms.y;
 #pragma unroll
-    for (int i = 0; i < DP / 8; i += 2) {
-      const float2 p = *(const float2*)(at + s * step + ch0 + i);
-      o[i] += w * p.x;
-      o[i + 1] += w * p.y;
+    for (int i = 0; i < DP / 8; i += 4) {
+      if (ch0 + i >= d.D) continue;
+      const f32x4 p = *(const f32x4*)(at + (((ch0 + i) >> 5) * 32 + row) * 32 + ((ch0 + i) & 31));
+#pragma unroll
+      for (int y = 0; y < 4; y++) o[i + y] = o[i + y] * keep + w * p[y];
     }
   }
-  win_few_store<E, DP / 8>(d, o, ch0, rr, hk, b, m, total, win_seq(d, b));
+  float all = m;
+#pragma unroll
+  for (int k = 8; k < 8 * SG; k <<= 1) all = fmaxf(all, __shfl_xor(all, k, 64));
+  const float w = m == -INFINITY ? 0.f : fast_exp2(m - all);
+  total *= w;
+#pragma unroll
+  for (int k = 8; k < 8 * SG; k <<= 1) total += __shfl_xor(total, k, 64);
+#pragma unroll
+  for (int i = 0; i < DP / 8; i++) {
+    o[i] *= w;
+#pragma unroll
+    for (int k = 8; k < 8 * SG; k <<= 1) o[i] += __shfl_xor(o[i], k, 64);
+  }
+  if (l < 8) win_few_store<E, DP / 8>(d, o, ch0, rr, hk, b, all, total, win_seq(d, b));
 }
 
 int window_attention_check(const WinDesc& d, bool backward, const char* what, bool sizes_only) {
@@ -415,12 +436,13 @@ static int win_fwd(const WinDesc& d, void* ws, hipStream_t st) {
   const long long rows = (long long)d.Sq * d.G, heads = (long long)d.Hk * d.B;
   const WinPlan p = win_plan(d);
   const WinShares sh = {p.shares, (float*)ws};
-  const dim3 few((unsigned)((rows + 31) / 32 * sh.n * heads)), many((unsigned)((rows + 127) / 128 * sh.n * heads)), join((unsigned)((rows * heads + 31) / 32));
+  const dim3 few((unsigned)((rows + 31) / 32 * sh.n * heads)), many((unsigned)((rows + 127) / 128 * sh.n * heads)), join4((unsigned)((rows * heads + 3) / 4)), join32((unsigned)((rows * heads + 31) / 32));
 #define GO(DP, NS, OCC)                                                                                                     \
   {                                                                                                                         \
     if (p.few) hipLaunchKernelGGL((win_few_kernel<E, DP>), few, dim3(256), 0, st, d, sh);                                   \
     else hipLaunchKernelGGL((win_fwd_kernel<E, DP, 4, NS, OCC>), many, dim3(256), 0, st, d, sh);                            \
-    if (sh.n > 1) hipLaunchKernelGGL((win_join_kernel<E, DP>), join, dim3(256), 0, st, d, sh);                              \
+    if (sh.n > 4) hipLaunchKernelGGL((win_join_kernel<E, DP, 8>), join4, dim3(256), 0, st, d, sh);                          \
+    else if (sh.n > 1) hipLaunchKernelGGL((win_join_kernel<E, DP, 1>), join32, dim3(256), 0, st, d, sh);                    \
   }
   if (d.D <= 32) GO(32, 3, 4) else if (d.D <= 64) GO(64, 3, 3) else GO(128, 2, 2)
 #undef GO
