@@ -452,14 +452,15 @@ static int win_fwd(const WinDesc& d, void* ws, hipStream_t st) {
 // workspace: the shares' sums
 size_t window_attention_fwd_workspace_bytes(const WinDesc& d) {
   if (window_attention_check(d, false, "window_attention_fwd", true)) return 0;
-  return win_shares_bytes(d) + 256;
+  const size_t n = win_shares_bytes(d);
+  return n ? n + 256 : 0;
 }
 
 int window_attention_fwd(const WinDesc& d, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
   if (int rc = window_attention_check(d, false, "window_attention_fwd")) return rc;
   if (d.B == 0 || d.Sq == 0) return SMBV_OK;
   const size_t need = window_attention_fwd_workspace_bytes(d);
-  if (need > 256 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255))) { set_error("window_attention_fwd: workspace short or not 256-byte aligned (%zu < %zu)", ws_bytes, need); return SMBV_ERR_WORKSPACE; }
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 255))) { set_error("window_attention_fwd: workspace short or not 256-byte aligned (%zu < %zu)", ws_bytes, need); return SMBV_ERR_WORKSPACE; }
   return dtype == 0 ? win_fwd<ElBf16>(d, ws, st) : win_fwd<ElF16>(d, ws, st);
 }
 

@@ -310,9 +310,53 @@ def colsum_bf16(X):
 
 
 # ---- operators of a transformer block over long token sequences: windowed attention with sinks, rotary positions with several axes, gated norms ------------
+# A call's checks and its C arguments but for the addresses follow from shapes, strides, types and numbers alone: they are worked out once for each such
+# signature (a call for one token is bound by what the host does for it: 38 -> 12 us).
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 _EL16 = {torch.bfloat16: 0, torch.float16: 1}
 _EL = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_PLANS = {}
+
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+class _Plan:
+    """One signature's C arguments without addresses; the entry point and its workspace's size once it has been called."""
+    __slots__ = ("args", "fn", "ws_bytes")
+
+    def __init__(self, args):
+        self.args, self.fn, self.ws_bytes = args, None, 0
+
+
+def _planned(key, make):
+    plan = _PLANS.get(key)
+    if plan is None:
+        if len(_PLANS) >= 1024:
+            _PLANS.clear()
+        plan = _PLANS[key] = _Plan(make())
+    return plan
+
+
+def _call(plan, name, args, device, workspace=True):
+    """The entry point on the tensors' device and the current stream."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _call(plan, name, args, device, workspace)
+    if plan.fn is None:
+        lib = _lib.load()
+        size = getattr(lib, name + "_workspace_bytes", None) if workspace else None
+        plan.ws_bytes = int(size(C.byref(args))) if size else 0
+        plan.fn = getattr(lib, name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if not workspace:
+        check(plan.fn(C.byref(args), stream), name)
+    elif plan.ws_bytes == 0:
+        check(plan.fn(C.byref(args), None, 0, stream), name)
+    else:
+        ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=device)
+        check(plan.fn(C.byref(args), ws.data_ptr(), plan.ws_bytes, stream), name)
 
 
 def _same_device(first, *ts):
@@ -324,6 +368,11 @@ def _same_device(first, *ts):
 def _ll3(t):
     """Strides of the first three dimensions (a dimension of one element has no stride to speak of)."""
     return _lib.c_ll3(*(0 if t.shape[i] <= 1 else t.stride(i) for i in range(3)))
+
+
+def _ll3_packed(shape):
+    _, r, h, c = shape
+    return _lib.c_ll3(r * h * c, h * c, c)
 
 
 def _heads4(t, name, shape, dtype):
@@ -342,7 +391,7 @@ def _extent(t):
 
 
 def _writable(t, name, inputs=()):
-    """An output's elements lie apart from each other and from every input."""
+    """A caller's output: its elements lie apart from each other and from every input."""
     span = 1
     for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
         if s < span:
@@ -373,11 +422,10 @@ def _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens):
             raise ValueError(f"{name}: a contiguous int32 tensor of {B} lengths")
     a = _lib.WindowAttn()
     a.dtype, a.B, a.Sq, a.Sk, a.H, a.Hk, a.Dh = _EL16[q.dtype], B, Sq, Sk, H, Hk, D
-    a.left, a.right = (min(max(int(x), -1), 2 ** 31 - 1) for x in (left, right))
-    if not 0 <= int(sinks) < 2 ** 31:
+    a.left, a.right = (min(max(x, -1), 2 ** 31 - 1) for x in (left, right))
+    if not 0 <= sinks < 2 ** 31:
         raise ValueError(f"sinks: {sinks}")
-    a.sinks, a.scale = int(sinks), float(D ** -0.5 if scale is None else scale)
-    a.q_lens, a.k_lens, a.q, a.k, a.v = _p(q_lens), _p(k_lens), _p(q), _p(k), _p(v)
+    a.sinks, a.scale = sinks, D ** -0.5 if scale is None else scale
     a.sq, a.sk, a.sv = _ll3(q), _ll3(k), _ll3(v)
     return a
 
@@ -389,23 +437,32 @@ def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_l
     up to 128).  Query i stands at position p = i + k_len - q_len and sees key j iff j < k_len, j <= p + right (right < 0: no bound; 0: causal) and
     (j >= p - left (left < 0: no bound) or j < sinks).  q_lens / k_lens: int32 [B] on the device (None: Sq / Sk), so the queries are the last rows of their
     sequence: all of them in training, the newest tokens against a cache in serving (Sq = 1).  A row that sees nothing, padded rows included, is 0 with lse -inf.
-    Keys that no row of a call can see are never read; a NaN or infinity in a value that SOME rows see can reach other rows near them.
+    Keys that no row of a call can see do not take part, whatever they hold; a NaN or infinity in a value that SOME rows see can reach other rows near them.
 
     Returns (o [B, Sq, H, D], lse fp32 [B, H, Sq]) and with ``resid`` also the residual of o's rounding, which window_attention_bwd takes as ``o_lo``.
     out: a tensor for o (its strides free; with ``resid`` the residual gets a tensor of the same strides)."""
-    a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
-    lib = _lib.load()
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    _need_gpu(o)
-    _same_device(q, o)
-    _heads4(o, "out", q.shape, q.dtype)
-    _writable(o, "out", (q, k, v))
+    left, right, sinks, scale = int(left), int(right), int(sinks), None if scale is None else float(scale)
+
+    def make():
+        a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
+        if out is not None:
+            _need_gpu(out)
+            _same_device(q, out)
+            _heads4(out, "out", q.shape, q.dtype)
+        a.so = _ll3_packed(q.shape) if out is None else _ll3(out)
+        return a
+
+    plan = _planned(("window_fwd", _meta(q), _meta(k), _meta(v), left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(out)), make)
+    if out is None:
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _writable(out, "out", (q, k, v))
+        o = out
     o_lo = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device) if resid else None
-    lse = torch.empty(a.B, a.H, a.Sq, dtype=torch.float32, device=q.device)
-    a.o, a.o_lo, a.lse, a.so = _p(o), _p(o_lo), _p(lse), _ll3(o)
-    with torch.cuda.device(q.device):
-        ws = _ws(lib.smbv_window_attention_fwd_workspace_bytes(C.byref(a)), q.device)
-        check(lib.smbv_window_attention_fwd(C.byref(a), _p(ws), ws.numel(), _stream()), "smbv_window_attention_fwd")
+    lse = torch.empty((plan.args.B, plan.args.H, plan.args.Sq), dtype=torch.float32, device=q.device)
+    a = _lib.WindowAttn.from_buffer_copy(plan.args)
+    a.q_lens, a.k_lens, a.q, a.k, a.v, a.o, a.o_lo, a.lse = _p(q_lens), _p(k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(o_lo), lse.data_ptr()
+    _call(plan, "smbv_window_attention_fwd", a, q.device)
     return (o, lse, o_lo) if resid else (o, lse)
 
 
@@ -413,30 +470,46 @@ def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, sca
     """Gradients (dq, dk, dv) of window_attention_fwd (the same keyword arguments; o, lse and o_lo as it returned them; do: the gradient of o, any strides).
     A key head's gradient is the sum over its query heads.  Every element is written; the same call gives the same bits.  out: three tensors for the
     gradients, for instance the column blocks of one packed gradient."""
-    a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
-    lib = _lib.load()
-    _need_gpu(o, do, lse, o_lo)
-    _same_device(q, o, do, lse, o_lo)
-    for name, t in (("o", o), ("do", do), ("o_lo", o_lo)):
-        if t is not None:
-            _heads4(t, name, q.shape, q.dtype)
-    if o_lo is not None and list(_ll3(o_lo)) != list(_ll3(o)):
-        raise ValueError("o_lo: the strides of o")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Sq) or not lse.is_contiguous():
-        raise ValueError(f"lse: a contiguous fp32 tensor of shape {(a.B, a.H, a.Sq)}")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)) if out is None else out
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        _need_gpu(t)
-        _same_device(q, t)
-        _heads4(t, name, like.shape, q.dtype)
-        _writable(t, name, (q, k, v, o, do, o_lo, lse))
-    if len({t.data_ptr() for t in (dq, dk, dv) if t.numel()}) < sum(t.numel() > 0 for t in (dq, dk, dv)):
-        raise ValueError("out: three tensors")
-    a.o, a.o_lo, a.lse, a.d_o, a.dq, a.dk, a.dv = _p(o), _p(o_lo), _p(lse), _p(do), _p(dq), _p(dk), _p(dv)
-    a.so, a.sdo, a.sdq, a.sdk, a.sdv = _ll3(o), _ll3(do), _ll3(dq), _ll3(dk), _ll3(dv)
-    with torch.cuda.device(q.device):
-        ws = _ws(lib.smbv_window_attention_bwd_workspace_bytes(C.byref(a)), q.device)
-        check(lib.smbv_window_attention_bwd(C.byref(a), _p(ws), ws.numel(), _stream()), "smbv_window_attention_bwd")
+    left, right, sinks, scale = int(left), int(right), int(sinks), None if scale is None else float(scale)
+    outs = (None,) * 3 if out is None else tuple(out)
+
+    def make():
+        a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
+        _need_gpu(o, do, lse, o_lo)
+        _same_device(q, o, do, lse, o_lo)
+        for name, t in (("o", o), ("do", do), ("o_lo", o_lo)):
+            if t is not None:
+                _heads4(t, name, q.shape, q.dtype)
+        if o_lo is not None and list(_ll3(o_lo)) != list(_ll3(o)):
+            raise ValueError("o_lo: the strides of o")
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Sq) or not lse.is_contiguous():
+            raise ValueError(f"lse: a contiguous fp32 tensor of shape {(a.B, a.H, a.Sq)}")
+        for name, t, like in zip(("dq", "dk", "dv"), outs, (q, k, v)):
+            if out is not None:
+                if t is None:
+                    raise ValueError("out: three tensors")
+                _need_gpu(t)
+                _same_device(q, t)
+                _heads4(t, name, like.shape, q.dtype)
+        a.so, a.sdo = _ll3(o), _ll3(do)
+        a.sdq, a.sdk, a.sdv = (_ll3_packed(like.shape) if t is None else _ll3(t) for t, like in zip(outs, (q, k, v)))
+        return a
+
+    key = ("window_bwd", _meta(q), _meta(k), _meta(v), _meta(o), _meta(do), _meta(lse), left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(o_lo),
+           out is None, *(_meta(t) for t in outs))
+    plan = _planned(key, make)
+    if out is None:
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    else:
+        dq, dk, dv = outs
+        for name, t in zip(("dq", "dk", "dv"), outs):
+            _writable(t, name, (q, k, v, o, do, o_lo, lse))
+        if len({t.data_ptr() for t in outs if t.numel()}) < sum(t.numel() > 0 for t in outs):
+            raise ValueError("out: three tensors")
+    a = _lib.WindowAttn.from_buffer_copy(plan.args)
+    a.q_lens, a.k_lens, a.q, a.k, a.v = _p(q_lens), _p(k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.o, a.o_lo, a.lse, a.d_o, a.dq, a.dk, a.dv = o.data_ptr(), _p(o_lo), lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    _call(plan, "smbv_window_attention_bwd", a, q.device)
     return dq, dk, dv
 
 
@@ -446,52 +519,63 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
     in order; inv_freq: fp32 [sum(sections)].  Pair p turns by pos[its axis] * inv_freq[p]; the first 2 * sum(sections) channels of a head are the pairs
     (p, p + sum(sections)), or (2p, 2p + 1) with ``interleaved``; the rest stays.  transpose: the inverse turn - what a gradient goes through on the way back.
     Returns (q', k'); out: tensors for them, (q, k) themselves to turn in place."""
-    _need_gpu(q, k, pos, inv_freq)
-    _same_device(q, k, pos, inv_freq)
-    if q.dtype not in _EL:
-        raise ValueError(f"rope_axes: bf16, fp16 or fp32, got {q.dtype}")
-    if q.dim() != 4:
-        raise ValueError(f"q: expected [B, S, H, D], got {tuple(q.shape)}")
-    B, S, H, D = q.shape
-    Hk = 0 if k is None else (k.shape[2] if k.dim() == 4 else -1)
-    _heads4(q, "q", (B, S, H, D), q.dtype)
-    if k is not None:
-        _heads4(k, "k", (B, S, Hk, D), q.dtype)
-    sections = [int(n) for n in sections]
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) <= 0 or 2 * sum(sections) > D:
-        raise ValueError(f"sections {sections}: one to four axes that own between them 1 .. {D // 2} pairs")
-    if pos.dtype not in (torch.int32, torch.int64) or tuple(pos.shape) not in ((len(sections), B, S), (len(sections), S)):
-        raise ValueError(f"pos: int32 or int64 of shape {(len(sections), B, S)} or {(len(sections), S)}, got {pos.dtype} {tuple(pos.shape)}")
-    if inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (sum(sections),) or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq: a contiguous fp32 tensor of {sum(sections)} frequencies")
-    lib = _lib.load()
-    qo, ko = (torch.empty(q.shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)) if out is None else out
-    for name, t, like, other in (("q", qo, q, k), ("k", ko, k, q)):
-        if (t is None) != (like is None):
-            raise ValueError("out: one tensor for each of q and k")
-        if t is None:
-            continue
-        _need_gpu(t)
-        _same_device(q, t)
-        _heads4(t, f"out of {name}", like.shape, q.dtype)
-        in_place = t.data_ptr() == like.data_ptr() and list(_ll3(t)) == list(_ll3(like))
-        # (in place beside the other operand's columns of one packed projection is fine: the elements are apart)
-        _writable(t, f"out of {name}", (pos, inv_freq) if in_place else (q, k, pos, inv_freq))
-    a = _lib.RopeAxesCfg()
-    a.dtype, a.B, a.S, a.H, a.Hk, a.Dh, a.axes = _EL[q.dtype], B, S, H, Hk, D, len(sections)
-    a.section = (C.c_int * 4)(*sections)
-    a.interleaved, a.transpose, a.pos64 = int(interleaved), int(transpose), int(pos.dtype == torch.int64)
-    a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = _p(q), _p(k), _p(qo), _p(ko), _p(pos), _p(inv_freq)
-    a.sq, a.sqo = _ll3(q), _ll3(qo)
-    if k is not None:
-        a.sk, a.sko = _ll3(k), _ll3(ko)
-    a.spos = _lib.c_ll3(pos.stride(0), pos.stride(1) if pos.dim() == 3 else 0, pos.stride(-1))
-    with torch.cuda.device(q.device):
-        check(lib.smbv_rope_axes(C.byref(a), _stream()), "smbv_rope_axes")
+    sections = tuple(int(n) for n in sections)
+    qo, ko = (None, None) if out is None else out
+
+    def make():
+        _need_gpu(q, k, pos, inv_freq)
+        _same_device(q, k, pos, inv_freq)
+        if q.dtype not in _EL:
+            raise ValueError(f"rope_axes: bf16, fp16 or fp32, got {q.dtype}")
+        if q.dim() != 4:
+            raise ValueError(f"q: expected [B, S, H, D], got {tuple(q.shape)}")
+        B, S, H, D = q.shape
+        Hk = 0 if k is None else (k.shape[2] if k.dim() == 4 else -1)
+        _heads4(q, "q", (B, S, H, D), q.dtype)
+        if k is not None:
+            _heads4(k, "k", (B, S, Hk, D), q.dtype)
+        if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) <= 0 or 2 * sum(sections) > D:
+            raise ValueError(f"sections {sections}: one to four axes that own between them 1 .. {D // 2} pairs")
+        if pos.dtype not in (torch.int32, torch.int64) or tuple(pos.shape) not in ((len(sections), B, S), (len(sections), S)):
+            raise ValueError(f"pos: int32 or int64 of shape {(len(sections), B, S)} or {(len(sections), S)}, got {pos.dtype} {tuple(pos.shape)}")
+        if inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (sum(sections),) or not inv_freq.is_contiguous():
+            raise ValueError(f"inv_freq: a contiguous fp32 tensor of {sum(sections)} frequencies")
+        a = _lib.RopeAxesCfg()
+        a.dtype, a.B, a.S, a.H, a.Hk, a.Dh, a.axes = _EL[q.dtype], B, S, H, Hk, D, len(sections)
+        a.section = (C.c_int * 4)(*sections)
+        a.interleaved, a.transpose, a.pos64 = int(interleaved), int(transpose), int(pos.dtype == torch.int64)
+        for name, t, like, s_in, s_out in (("q", qo, q, "sq", "sqo"), ("k", ko, k, "sk", "sko")):
+            if out is not None and (t is None) != (like is None):
+                raise ValueError("out: one tensor for each of q and k")
+            if like is None:
+                continue
+            setattr(a, s_in, _ll3(like))
+            setattr(a, s_out, _ll3_packed(like.shape) if t is None else _ll3(t))
+            if t is not None:
+                _need_gpu(t)
+                _same_device(q, t)
+                _heads4(t, f"out of {name}", like.shape, q.dtype)
+        a.spos = _lib.c_ll3(pos.stride(0), pos.stride(1) if pos.dim() == 3 else 0, pos.stride(-1))
+        return a
+
+    plan = _planned(("rope_axes", _meta(q), _meta(k), _meta(pos), _meta(inv_freq), sections, bool(interleaved), bool(transpose), out is None, _meta(qo), _meta(ko)), make)
+    if out is None:
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        for name, t, like in (("q", qo, q), ("k", ko, k)):
+            if t is not None:
+                in_place = t.data_ptr() == like.data_ptr() and list(_ll3(t)) == list(_ll3(like))
+                # (in place beside the other operand's columns of one packed projection is fine: the elements are apart)
+                _writable(t, f"out of {name}", (pos, inv_freq) if in_place else (q, k, pos, inv_freq))
+    a = _lib.RopeAxesCfg.from_buffer_copy(plan.args)
+    a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), pos.data_ptr(), inv_freq.data_ptr()
+    _call(plan, "smbv_rope_axes", a, q.device, workspace=False)
     return qo, ko
 
 
 def _rows2(t, name, lead, d, dtype):
+    """The stride between the rows of t [*lead, d]."""
     if t.dtype != dtype or tuple(t.shape) != (*lead, d):
         raise ValueError(f"{name}: expected {dtype} {(*lead, d)}, got {t.dtype} {tuple(t.shape)}")
     if d > 1 and t.stride(-1) != 1:
@@ -500,7 +584,7 @@ def _rows2(t, name, lead, d, dtype):
         r = t.view(-1, d) if t.numel() else t.reshape(0, d)
     except RuntimeError:
         raise ValueError(f"{name}: the leading dimensions must have one stride between rows") from None
-    return r, (r.stride(0) if r.shape[0] > 1 else d)
+    return r.stride(0) if r.shape[0] > 1 else d
 
 
 def _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps):
@@ -514,13 +598,13 @@ def _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pr
         raise ValueError(f"h: rows of at least one element, got {tuple(h.shape)}")
     d, lead = h.shape[-1], tuple(h.shape[:-1])
     a = _lib.GatedNorm()
-    hr, a.ldh = _rows2(h, "h", lead, d, h.dtype)
-    xr, a.ldx = _rows2(x, "x", lead, d, x.dtype)
-    rows = hr.shape[0]
+    a.ldh = _rows2(h, "h", lead, d, h.dtype)
+    a.ldx = _rows2(x, "x", lead, d, x.dtype)
+    rows = h.numel() // d
     for name, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)):
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (d,) or not t.is_contiguous()):
             raise ValueError(f"{name}: a contiguous fp32 tensor of {d} elements")
-    a.h_type, a.x_type, a.d, a.post, a.pre, a.eps, a.res_scale, a.rows = _EL[h.dtype], _EL[x.dtype], d, _NORMS[post], _NORMS[pre], float(eps), float(res_scale), rows
+    a.h_type, a.x_type, a.d, a.post, a.pre, a.eps, a.res_scale, a.rows = _EL[h.dtype], _EL[x.dtype], d, _NORMS[post], _NORMS[pre], eps, res_scale, rows
     a.rows_per_gate = max(rows, 1)
     if gate is not None:
         if gate.dtype != torch.float32 or gate.dim() < 1 or gate.shape[-1] != d or not gate.is_contiguous():
@@ -533,8 +617,7 @@ def _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pr
             raise ValueError(f"gate {tuple(gate.shape)}: one row, or one for each of h's leading dimensions {lead}")
         if groups:
             a.rows_per_gate = max(rows // groups, 1)
-    a.h, a.x, a.post_w, a.post_b, a.gate, a.pre_w, a.pre_b = _p(hr), _p(xr), _p(post_w), _p(post_b), _p(gate), _p(pre_w), _p(pre_b)
-    return a, lead, d, rows
+    return a, lead, d
 
 
 def gated_norm_fwd(h, x, *, post="rms", post_w=None, post_b=None, gate=None, res_scale=1.0, pre="rms", pre_w=None, pre_b=None, eps=1e-6, out=None):
@@ -547,29 +630,35 @@ def gated_norm_fwd(h, x, *, post="rms", post_w=None, post_b=None, gate=None, res
     [n, d] whose n divides the rows: one gate for rows / n consecutive rows).  y is formed from x1 before its rounding.  Rows up to 8192 wide.
 
     Returns (x1 in x's type, y in h's type or None without ``pre``, stats fp32 [rows, 4] for gated_norm_bwd).  out: (x1, y), x1 may be x itself."""
-    a, lead, d, rows = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
-    lib = _lib.load()
+    eps, res_scale = float(eps), float(res_scale)
+    x1, y = (None, None) if out is None else out
+
+    def make():
+        a, lead, d = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
+        if out is not None:
+            if (y is None) != (pre is None):
+                raise ValueError("out: (x1, y), y None exactly when there is no norm in front of the next block")
+            _need_gpu(x1, y)
+            _same_device(h, x1, y)
+        a.ldx1 = d if x1 is None else _rows2(x1, "x1", lead, d, x.dtype)
+        a.ldy = d if y is None else _rows2(y, "y", lead, d, h.dtype)
+        return a
+
+    plan = _planned(("gated_norm_fwd", _meta(h), _meta(x), post, _meta(post_w), _meta(post_b), _meta(gate), res_scale, pre, _meta(pre_w), _meta(pre_b), eps,
+                         out is None, _meta(x1), _meta(y)), make)
     if out is None:
-        x1 = torch.empty((*lead, d), dtype=x.dtype, device=h.device)
-        y = torch.empty((*lead, d), dtype=h.dtype, device=h.device) if pre else None
+        x1 = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty(h.shape, dtype=h.dtype, device=h.device) if pre else None
     else:
-        x1, y = out
-        if (y is None) != (pre is None):
-            raise ValueError("out: (x1, y), y None exactly when there is no norm in front of the next block")
-        _need_gpu(x1, y)
-        _same_device(h, x1, y)
-    x1r, a.ldx1 = _rows2(x1, "x1", lead, d, x.dtype)
-    params = (h, post_w, post_b, gate, pre_w, pre_b)
-    _writable(x1, "x1", params if x1.data_ptr() == x.data_ptr() and a.ldx1 == a.ldx else (*params, x))
-    a.x1 = _p(x1r)
-    if y is not None:
-        yr, a.ldy = _rows2(y, "y", lead, d, h.dtype)
-        _writable(y, "y", (*params, x, x1))
-        a.y = _p(yr)
-    stats = torch.empty(rows, 4, dtype=torch.float32, device=h.device)
-    a.stats = _p(stats)
-    with torch.cuda.device(h.device):
-        check(lib.smbv_gated_norm_fwd(C.byref(a), _stream()), "smbv_gated_norm_fwd")
+        params = (h, post_w, post_b, gate, pre_w, pre_b)
+        _writable(x1, "x1", params if x1.data_ptr() == x.data_ptr() and plan.args.ldx1 == plan.args.ldx else (*params, x))
+        if y is not None:
+            _writable(y, "y", (*params, x, x1))
+    stats = torch.empty((plan.args.rows, 4), dtype=torch.float32, device=h.device)
+    a = _lib.GatedNorm.from_buffer_copy(plan.args)
+    a.h, a.x, a.post_w, a.post_b, a.gate, a.pre_w, a.pre_b = h.data_ptr(), x.data_ptr(), _p(post_w), _p(post_b), _p(gate), _p(pre_w), _p(pre_b)
+    a.x1, a.y, a.stats = x1.data_ptr(), _p(y), stats.data_ptr()
+    _call(plan, "smbv_gated_norm_fwd", a, h.device, workspace=False)
     return x1, y, stats
 
 
@@ -577,36 +666,40 @@ def gated_norm_bwd(dx1, dy, h, x, stats, *, post="rms", post_w=None, post_b=None
     """Gradients of gated_norm_fwd (the same keyword arguments; h, x: its inputs; stats as it returned them).  dx1: the gradient that reaches x1 from elsewhere
     (x's type, or None), dy: that of y (h's type; None without ``pre``).  Returns a dict: "dh", "dx" and, for every parameter that was given, its fp32
     gradient under its name ("gate", "post_w", "post_b", "pre_w", "pre_b"; None for the others).  The same call gives the same bits.  out: (dh, dx)."""
-    a, lead, d, rows = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, 0.0)
-    lib = _lib.load()
-    _need_gpu(dx1, dy, stats)
-    _same_device(h, dx1, dy, stats)
-    if (dy is None) != (pre is None) or (dx1 is None and dy is None):
-        raise ValueError("dy: given exactly when there is a norm in front of the next block; without it dx1 is needed")
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 4) or not stats.is_contiguous():
-        raise ValueError(f"stats: a contiguous fp32 tensor of shape {(rows, 4)}")
-    if dx1 is not None:
-        dx1r, a.lddx1 = _rows2(dx1, "dx1", lead, d, x.dtype)
-        a.dx1 = _p(dx1r)
-    if dy is not None:
-        dyr, a.lddy = _rows2(dy, "dy", lead, d, h.dtype)
-        a.dy = _p(dyr)
-    a.stats = _p(stats)
-    dh, dx = (torch.empty((*lead, d), dtype=h.dtype, device=h.device), torch.empty((*lead, d), dtype=x.dtype, device=h.device)) if out is None else out
-    _need_gpu(dh, dx)
-    _same_device(h, dh, dx)
-    dhr, a.lddh = _rows2(dh, "dh", lead, d, h.dtype)
-    dxr, a.lddx = _rows2(dx, "dx", lead, d, x.dtype)
-    ins = (h, x, dx1, dy, stats, post_w, post_b, gate, pre_w, pre_b)
-    _writable(dh, "dh", (*ins, dx))
-    _writable(dx, "dx", ins)
-    a.dh, a.dx = _p(dhr), _p(dxr)
-    new = torch.empty_like if rows else torch.zeros_like  # (no rows: nothing is launched, the sums are empty)
+    res_scale = float(res_scale)
+    dh, dx = (None, None) if out is None else out
+
+    def make():
+        a, lead, d = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, 0.0)
+        _need_gpu(dx1, dy, stats, dh, dx)
+        _same_device(h, dx1, dy, stats, dh, dx)
+        if (dy is None) != (pre is None) or (dx1 is None and dy is None):
+            raise ValueError("dy: given exactly when there is a norm in front of the next block; without it dx1 is needed")
+        if stats.dtype != torch.float32 or tuple(stats.shape) != (a.rows, 4) or not stats.is_contiguous():
+            raise ValueError(f"stats: a contiguous fp32 tensor of shape {(a.rows, 4)}")
+        if dx1 is not None:
+            a.lddx1 = _rows2(dx1, "dx1", lead, d, x.dtype)
+        if dy is not None:
+            a.lddy = _rows2(dy, "dy", lead, d, h.dtype)
+        a.lddh = d if out is None else _rows2(dh, "dh", lead, d, h.dtype)
+        a.lddx = d if out is None else _rows2(dx, "dx", lead, d, x.dtype)
+        return a
+
+    plan = _planned(("gated_norm_bwd", _meta(dx1), _meta(dy), _meta(h), _meta(x), _meta(stats), post, _meta(post_w), _meta(post_b), _meta(gate), res_scale,
+                                   pre, _meta(pre_w), _meta(pre_b), out is None, _meta(dh), _meta(dx)), make)
+    if out is None:
+        dh, dx = torch.empty(h.shape, dtype=h.dtype, device=h.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        ins = (h, x, dx1, dy, stats, post_w, post_b, gate, pre_w, pre_b)
+        _writable(dh, "dh", (*ins, dx))
+        _writable(dx, "dx", ins)
+    new = torch.empty_like if plan.args.rows else torch.zeros_like  # (no rows: nothing is launched, the sums are empty)
     gr = {n: None if t is None else new(t) for n, t in (("gate", gate), ("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b))}
+    a = _lib.GatedNorm.from_buffer_copy(plan.args)
+    a.h, a.x, a.post_w, a.post_b, a.gate, a.pre_w, a.pre_b = h.data_ptr(), x.data_ptr(), _p(post_w), _p(post_b), _p(gate), _p(pre_w), _p(pre_b)
+    a.dx1, a.dy, a.stats, a.dh, a.dx = _p(dx1), _p(dy), stats.data_ptr(), dh.data_ptr(), dx.data_ptr()
     a.dgate, a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_p(gr[n]) for n in ("gate", "post_w", "post_b", "pre_w", "pre_b"))
-    with torch.cuda.device(h.device):
-        ws = _ws(lib.smbv_gated_norm_bwd_workspace_bytes(C.byref(a)), h.device)
-        check(lib.smbv_gated_norm_bwd(C.byref(a), _p(ws), ws.numel(), _stream()), "smbv_gated_norm_bwd")
+    _call(plan, "smbv_gated_norm_bwd", a, h.device)
     return {"dh": dh, "dx": dx, **gr}
 
 
