@@ -4,210 +4,232 @@
 //     t  = dx1 + pre^T(dy),   dx = res_scale t,   dgate = sum t n,   dh = post^T(gate t),   dpost_w = sum gate t hhat,  dpre_w = sum dy xhat, ...
 //     norm^T(g) with z = w g:  (z - [LayerNorm: mean z] - hat mean(z hat)) / deviation
 // Bound by HBM: the forward reads h, x and writes x1, y; the backward reads dx1, dy, h, x (x1 is formed again from h and x in 32 bits rather than read back
-// rounded) and writes dh, dx.  A row lives in the registers of 1, 2 or 4 waves; sums and statistics are fp32, variances about the mean.
+// rounded) and writes dh, dx.  A row lives in the registers of K waves, 8 elements a lane (12 where that spares a second wave: 768): what the backward keeps
+// beside a row - three parameters and four sums a column - then leaves four waves a SIMD (with 16 a lane it spilled: 184 us instead of 64 at 20,480 x 768).
+// A workgroup walks rows with the parameters in registers.  Sums and statistics are fp32, variances about the mean.
 // The parameters' gradients: every workgroup owns a run of rows and adds its rows' terms in registers; a second launch adds the workgroups' sums in a fixed
-// order (no float atomics: the result repeats bit for bit).
+// order (no float atomics: the result repeats bit for bit).  Within a gate's rows sum t n = post_w sum t hhat + post_b sum t, and the same two sums times the gate
+// are dpost_w and dpost_b.
 #include "smbv_common.h"
 #include "smbv_kernels.h"
 #include <math.h>
 
 namespace smbv {
 
-template <class T, int V> struct __attribute__((aligned(V > 1 ? (sizeof(T) * V > 16 ? 16 : sizeof(T) * V) : sizeof(T)))) GnVec { T e[V]; };
+// V elements of a row at once.  WIDE: rows start on 16 bytes and end on a whole vector; otherwise the vector is read where it lies (the memory takes any
+// alignment) and the row's last one element by element.
+template <class T, int V, bool WIDE> struct __attribute__((packed, aligned(WIDE ? (sizeof(T) * V > 16 ? 16 : sizeof(T) * V) : sizeof(T)))) GnVec { T e[V]; };
 
 // the row's elements of this lane: NE of them in vectors of V, vector i at column (i LANES + lane) V; past the row's end zeros
-template <class T, int NE, int V, int LANES>
+template <class T, int NE, int V, int LANES, bool WIDE>
 __device__ __forceinline__ void gn_load(float (&f)[NE], const T* p, int lane, int d, bool on) {
 #pragma unroll
   for (int i = 0; i < NE / V; i++) {
     const int c = (i * LANES + lane) * V;
-    if (on && c < d) {
-      const GnVec<T, V> v = *(const GnVec<T, V>*)(p + c);
+    if (on && c + (WIDE ? 1 : V) <= d) {
+      const GnVec<T, V, WIDE> v = *(const GnVec<T, V, WIDE>*)(p + c);
 #pragma unroll
       for (int e = 0; e < V; e++) f[i * V + e] = (float)v.e[e];
     } else {
 #pragma unroll
       for (int e = 0; e < V; e++) f[i * V + e] = 0.f;
+      if constexpr (!WIDE) {
+        if (on && c < d) {
+#pragma unroll
+          for (int e = 0; e < V; e++)
+            if (c + e < d) f[i * V + e] = (float)p[c + e];
+        }
+      }
     }
   }
 }
-template <class T, int NE, int V, int LANES>
+template <class T, int NE, int V, int LANES, bool WIDE>
 __device__ __forceinline__ void gn_store(const float (&f)[NE], T* p, int lane, int d) {
 #pragma unroll
   for (int i = 0; i < NE / V; i++) {
     const int c = (i * LANES + lane) * V;
-    if (c < d) {
-      GnVec<T, V> v;
+    if (c + (WIDE ? 1 : V) <= d) {
+      GnVec<T, V, WIDE> v;
 #pragma unroll
       for (int e = 0; e < V; e++) v.e[e] = (T)f[i * V + e];
-      *(GnVec<T, V>*)(p + c) = v;
+      *(GnVec<T, V, WIDE>*)(p + c) = v;
+    } else if constexpr (!WIDE) {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (c + e < d) p[c + e] = (T)f[i * V + e];
     }
   }
 }
-template <int NE, int V, int LANES>
+template <int NE, int V, int LANES, bool WIDE>
 __device__ __forceinline__ void gn_param(float (&f)[NE], const float* p, float none, int lane, int d) {
-  if (p) gn_load<float, NE, V, LANES>(f, p, lane, d, true);
+  if (p) gn_load<float, NE, V, LANES, WIDE>(f, p, lane, d, true);
   else {
 #pragma unroll
     for (int i = 0; i < NE; i++) f[i] = none;
   }
 }
 // is register i of this lane inside the row
-template <int V, int LANES> __device__ __forceinline__ bool gn_in(int i, int lane, int d) { return ((i / V) * LANES + lane) * V < d; }
+template <int V, int LANES, bool WIDE> __device__ __forceinline__ bool gn_in(int i, int lane, int d) {
+  return ((i / V) * LANES + lane) * V + (WIDE ? 0 : i % V) < d;
+}
 
 // sums over a row's K waves; every wave of the workgroup calls it the same number of times (two alternating slots: one barrier a call)
-template <int K, int N>
+template <int K, int WAVES>
 struct GnReduce {
-  float* slots;  // LDS [2][4 waves][N]
+  float* slots;  // LDS [2][waves][2]
   int flip;
+  template <int N>
   __device__ __forceinline__ void operator()(float (&s)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) s[i] = wave_sum(s[i]);
     if constexpr (K > 1) {
       const int w = threadIdx.x >> 6, l = threadIdx.x & 63, w0 = w & ~(K - 1);
-      float* at = slots + flip * 4 * N;
+      float* at = slots + flip * WAVES * 2;
       if (l == 0) {
 #pragma unroll
-        for (int i = 0; i < N; i++) at[w * N + i] = s[i];
+        for (int i = 0; i < N; i++) at[w * 2 + i] = s[i];
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < N; i++) {
         s[i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; k++) s[i] += at[(w0 + k) * N + i];
+        for (int k = 0; k < K; k++) s[i] += at[(w0 + k) * 2 + i];
       }
       flip ^= 1;
     }
   }
 };
 
-template <int NE, int V, int LANES, int K>
-__device__ __forceinline__ void gn_stats(const float (&f)[NE], int kind, int lane, int d, float eps, float& mu, float& rs, GnReduce<K, 2>& red) {
+template <int NE, int V, int LANES, bool WIDE, class R>
+__device__ __forceinline__ void gn_stats(const float (&f)[NE], int kind, int lane, int d, float eps, float& mu, float& rs, R& red) {
   mu = 0.f;
   if (kind == 2) {
-    float s[2] = {0.f, 0.f};
+    float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NE; i++) s[0] += f[i];
     red(s);
     mu = s[0] / d;
   }
-  float q[2] = {0.f, 0.f};
+  float q[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < NE; i++) {
-    const float c = gn_in<V, LANES>(i, lane, d) ? f[i] - mu : 0.f;
+    const float c = gn_in<V, LANES, WIDE>(i, lane, d) ? f[i] - mu : 0.f;
     q[0] += c * c;
   }
   red(q);
   rs = 1.0f / sqrtf(q[0] / d + eps);
 }
 
-template <class TH, class TX, int NE, int V, int K>
-__global__ __launch_bounds__(256) void gated_norm_fwd_kernel(GatedNormDesc d) {
-  constexpr int LANES = 64 * K, TEAMS = 4 / K;
-  __shared__ float slots[2 * 4 * 2];
-  const int lane = threadIdx.x & (LANES - 1), team = threadIdx.x / LANES;
-  const long long row = (long long)blockIdx.x * TEAMS + team;
-  const bool on = row < d.rows;
-  GnReduce<K, 2> red{slots, 0};
-  float h[NE], x[NE], w[NE];
-  gn_load<TH, NE, V, LANES>(h, (const TH*)d.h + row * d.ldh, lane, d.d, on);
-  gn_load<TX, NE, V, LANES>(x, (const TX*)d.x + row * d.ldx, lane, d.d, on);
-  float mu = 0.f, rs = 1.f;
-  if (d.post) {
-    gn_stats<NE, V, LANES, K>(h, d.post, lane, d.d, d.eps, mu, rs, red);
-    float b[NE];
-    gn_param<NE, V, LANES>(w, d.post_w, 1.f, lane, d.d);
-    gn_param<NE, V, LANES>(b, d.post_b, 0.f, lane, d.d);
+// a workgroup has 4 waves, or the 8 or 16 that one row takes
+template <class TH, class TX, int NE, int V, int K, bool WIDE>
+__global__ __launch_bounds__(K > 4 ? 64 * K : 256) void gated_norm_fwd_kernel(GatedNormDesc d) {
+  constexpr int LANES = 64 * K, WAVES = K > 4 ? K : 4, TEAMS = WAVES / K;
+  __shared__ float slots[2 * WAVES * 2];
+  const int lane = threadIdx.x & (LANES - 1), team = __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+  GnReduce<K, WAVES> red{slots, 0};
+  float w[NE], b[NE], gt[NE], pw[NE], pb[NE];
+  gn_param<NE, V, LANES, WIDE>(w, d.post_w, 1.f, lane, d.d);
+  gn_param<NE, V, LANES, WIDE>(b, d.post_b, 0.f, lane, d.d);
+  gn_param<NE, V, LANES, WIDE>(pw, d.pre_w, 1.f, lane, d.d);
+  gn_param<NE, V, LANES, WIDE>(pb, d.pre_b, 0.f, lane, d.d);
+  gn_param<NE, V, LANES, WIDE>(gt, nullptr, 1.f, lane, d.d);
+  long long g = -1;
+  for (long long base = (long long)blockIdx.x * TEAMS; base < d.rows; base += (long long)gridDim.x * TEAMS) {
+    const long long row = base + team;
+    const bool on = row < d.rows;
+    float h[NE], x[NE];
+    gn_load<TH, NE, V, LANES, WIDE>(h, (const TH*)d.h + row * d.ldh, lane, d.d, on);
+    gn_load<TX, NE, V, LANES, WIDE>(x, (const TX*)d.x + row * d.ldx, lane, d.d, on);
+    if (d.gate && on && row / d.rows_per_gate != g) {
+      g = row / d.rows_per_gate;
+      gn_load<float, NE, V, LANES, WIDE>(gt, d.gate + g * d.d, lane, d.d, true);
+    }
+    float mu = 0.f, rs = 1.f;
+    if (d.post) {
+      gn_stats<NE, V, LANES, WIDE>(h, d.post, lane, d.d, d.eps, mu, rs, red);
 #pragma unroll
-    for (int i = 0; i < NE; i++) h[i] = (h[i] - mu) * rs * w[i] + b[i];
+      for (int i = 0; i < NE; i++) h[i] = (h[i] - mu) * rs * w[i] + b[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NE; i++) x[i] = gn_in<V, LANES, WIDE>(i, lane, d.d) ? __builtin_fmaf(d.res_scale, x[i], h[i] * gt[i]) : 0.f;
+    if (on) gn_store<TX, NE, V, LANES, WIDE>(x, (TX*)d.x1 + row * d.ldx1, lane, d.d);
+    float mx = 0.f, rx = 1.f;
+    if (d.pre) {
+      gn_stats<NE, V, LANES, WIDE>(x, d.pre, lane, d.d, d.eps, mx, rx, red);
+#pragma unroll
+      for (int i = 0; i < NE; i++) x[i] = (x[i] - mx) * rx * pw[i] + pb[i];
+      if (on) gn_store<TH, NE, V, LANES, WIDE>(x, (TH*)d.y + row * d.ldy, lane, d.d);
+    }
+    if (on && lane == 0) *(f32x4*)(d.stats + 4 * row) = (f32x4){mu, rs, mx, rx};
   }
-  if (d.gate) {
-    gn_param<NE, V, LANES>(w, d.gate + (on ? row / d.rows_per_gate : 0) * d.d, 1.f, lane, d.d);
-#pragma unroll
-    for (int i = 0; i < NE; i++) h[i] *= w[i];
-  }
-#pragma unroll
-  for (int i = 0; i < NE; i++) x[i] = gn_in<V, LANES>(i, lane, d.d) ? __builtin_fmaf(d.res_scale, x[i], h[i]) : 0.f;
-  if (on) gn_store<TX, NE, V, LANES>(x, (TX*)d.x1 + row * d.ldx1, lane, d.d);
-  float mx = 0.f, rx = 1.f;
-  if (d.pre) {
-    gn_stats<NE, V, LANES, K>(x, d.pre, lane, d.d, d.eps, mx, rx, red);
-    float b[NE];
-    gn_param<NE, V, LANES>(w, d.pre_w, 1.f, lane, d.d);
-    gn_param<NE, V, LANES>(b, d.pre_b, 0.f, lane, d.d);
-#pragma unroll
-    for (int i = 0; i < NE; i++) x[i] = (x[i] - mx) * rx * w[i] + b[i];
-    if (on) gn_store<TH, NE, V, LANES>(x, (TH*)d.y + row * d.ldy, lane, d.d);
-  }
-  if (on && lane == 0) *(f32x4*)(d.stats + 4 * row) = (f32x4){mu, rs, mx, rx};
 }
 
 // workspace of the backward: sums of C workgroups, [C][d] each: pre_w | pre_b | post_w | post_b, then the gate's, [C + gates][d]
 struct GnPart { float* base; int C; long long chunk; };
 
-template <class TH, class TX, int NE, int V, int K>
-__global__ __launch_bounds__(256, NE > 16 ? 1 : 2) void gated_norm_bwd_kernel(GatedNormDesc d, GnPart part) {
-  constexpr int LANES = 64 * K, TEAMS = 4 / K;
-  __shared__ float slots[2 * 4 * 2];
-  __shared__ float fold[TEAMS > 1 ? (TEAMS - 1) * LANES * NE : 1];
-  const int lane = threadIdx.x & (LANES - 1), team = threadIdx.x / LANES;
-  GnReduce<K, 2> red{slots, 0};
+template <class TH, class TX, int NE, int V, int K, bool WIDE, bool PER_ROW>
+__global__ __launch_bounds__(K > 4 ? 64 * K : 256) __attribute__((amdgpu_waves_per_eu(NE > 8 ? 3 : 4))) void gated_norm_bwd_kernel(GatedNormDesc d, GnPart part) {
+  constexpr int LANES = 64 * K, WAVES = K > 4 ? K : 4, TEAMS = WAVES / K;
+  __shared__ float slots[2 * WAVES * 2];
+  __shared__ float fold[2 * NE * 64 * WAVES];   // the teams' sums on their way out; between a workgroup's runs of rows: its sums for post_w, post_b
+  const int tid = threadIdx.x, lane = tid & (LANES - 1), team = __builtin_amdgcn_readfirstlane(tid / LANES);
+  GnReduce<K, WAVES> red{slots, 0};
   const long long c0 = blockIdx.x * part.chunk, c1 = c0 + part.chunk < d.rows ? c0 + part.chunk : d.rows;
-  const bool per_row = d.gate && d.rows_per_gate == 1;
-  float sw[NE], sb[NE], qw[NE], qb[NE], sg[NE];  // pre_w, pre_b, post_w, post_b, gate
+  float sw[NE], sb[NE], pw[NE];   // sums for pre_w, pre_b
 #pragma unroll
-  for (int i = 0; i < NE; i++) { sw[i] = 0.f; sb[i] = 0.f; qw[i] = 0.f; qb[i] = 0.f; }
-  // the teams' sums into one row of the workspace (team 0 writes)
+  for (int i = 0; i < NE; i++) { sw[i] = 0.f; sb[i] = 0.f; fold[i * 64 * WAVES + tid] = 0.f; fold[(NE + i) * 64 * WAVES + tid] = 0.f; }
+  gn_param<NE, V, LANES, WIDE>(pw, d.pre_w, 1.f, lane, d.d);
+  // the teams' sums of a column, in their order, and out by team 0
   auto flush = [&](float (&s)[NE], float* out) __attribute__((always_inline)) {
     if constexpr (TEAMS > 1) {
       __syncthreads();
-      if (team > 0) {
 #pragma unroll
-        for (int i = 0; i < NE; i++) fold[((team - 1) * NE + i) * LANES + lane] = s[i];
-      }
+      for (int i = 0; i < NE; i++) fold[i * 64 * WAVES + tid] = s[i];
       __syncthreads();
       if (team == 0) {
-        for (int k = 0; k < TEAMS - 1; k++)
+        for (int k = 1; k < TEAMS; k++)
 #pragma unroll
-          for (int i = 0; i < NE; i++) s[i] += fold[(k * NE + i) * LANES + lane];
+          for (int i = 0; i < NE; i++) s[i] += fold[i * 64 * WAVES + k * LANES + lane];
       }
     }
-    if (team == 0) gn_store<float, NE, V, LANES>(s, out, lane, d.d);
+    if (team == 0) gn_store<float, NE, V, LANES, WIDE>(s, out, lane, d.d);
   };
-  const long long rpg = d.gate && !per_row ? d.rows_per_gate : d.rows;
+  const bool gated = d.gate && !PER_ROW;
+  const long long rpg = gated ? d.rows_per_gate : d.rows;
   for (long long s0 = c0; s0 < c1;) {   // runs of rows with one gate
     const long long g = s0 / rpg, s1 = (g + 1) * rpg < c1 ? (g + 1) * rpg : c1;
-    float gt[NE];
-    if (!per_row) gn_param<NE, V, LANES>(gt, d.gate ? d.gate + g * d.d : nullptr, 1.f, lane, d.d);
+    float gw[NE], gb[NE], sa[NE], sc[NE];   // gate post_w, gate post_b; sums of t hhat and t over these rows
+    {
+      float w[NE];
+      gn_param<NE, V, LANES, WIDE>(gw, gated ? d.gate + g * d.d : nullptr, 1.f, lane, d.d);
+      gn_param<NE, V, LANES, WIDE>(gb, d.post_b, 0.f, lane, d.d);
+      gn_param<NE, V, LANES, WIDE>(w, d.post_w, 1.f, lane, d.d);
 #pragma unroll
-    for (int i = 0; i < NE; i++) sg[i] = 0.f;
+      for (int i = 0; i < NE; i++) { gb[i] *= gw[i]; gw[i] *= w[i]; sa[i] = 0.f; sc[i] = 0.f; }
+    }
     for (long long base = s0; base < s1; base += TEAMS) {
       const long long row = base + team;
       const bool on = row < s1;
       f32x4 st = {0.f, 0.f, 0.f, 0.f};
       if (on) st = *(const f32x4*)(d.stats + 4 * row);
-      float h[NE], x[NE], t[NE], dy[NE], w[NE];
-      gn_load<TH, NE, V, LANES>(h, (const TH*)d.h + row * d.ldh, lane, d.d, on);
-      gn_load<TX, NE, V, LANES>(x, (const TX*)d.x + row * d.ldx, lane, d.d, on);
-      gn_load<TX, NE, V, LANES>(t, (const TX*)d.dx1 + row * d.lddx1, lane, d.d, on && d.dx1);
-      if (per_row) gn_param<NE, V, LANES>(gt, on ? d.gate + row * d.d : nullptr, 1.f, lane, d.d);
-      float n[NE];
-      gn_param<NE, V, LANES>(w, d.post_w, 1.f, lane, d.d);
-      float b[NE];
-      gn_param<NE, V, LANES>(b, d.post_b, 0.f, lane, d.d);
+      float h[NE], x[NE], t[NE], dy[NE], gr[PER_ROW ? NE : 1];
+      gn_load<TH, NE, V, LANES, WIDE>(h, (const TH*)d.h + row * d.ldh, lane, d.d, on);
+      gn_load<TX, NE, V, LANES, WIDE>(x, (const TX*)d.x + row * d.ldx, lane, d.d, on && d.pre);
+      gn_load<TH, NE, V, LANES, WIDE>(dy, (const TH*)d.dy + row * d.lddy, lane, d.d, on && d.pre);
+      gn_load<TX, NE, V, LANES, WIDE>(t, (const TX*)d.dx1 + row * d.lddx1, lane, d.d, on && d.dx1);
+      if constexpr (PER_ROW) gn_load<float, NE, V, LANES, WIDE>(gr, d.gate + row * d.d, lane, d.d, on);
+      if (d.post) {
 #pragma unroll
-      for (int i = 0; i < NE; i++) {
-        if (d.post) h[i] = gn_in<V, LANES>(i, lane, d.d) ? (h[i] - st[0]) * st[1] : 0.f;   // hhat
-        n[i] = d.post ? h[i] * w[i] + b[i] : h[i];
+        for (int i = 0; i < NE; i++) h[i] = gn_in<V, LANES, WIDE>(i, lane, d.d) ? (h[i] - st[0]) * st[1] : 0.f;   // hhat
       }
       if (d.pre) {
-        gn_load<TH, NE, V, LANES>(dy, (const TH*)d.dy + row * d.lddy, lane, d.d, on);
-        float s[2] = {0.f, 0.f}, pw[NE];
-        gn_param<NE, V, LANES>(pw, d.pre_w, 1.f, lane, d.d);
+        float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NE; i++) {
-          x[i] = gn_in<V, LANES>(i, lane, d.d) ? (__builtin_fmaf(d.res_scale, x[i], gt[i] * n[i]) - st[2]) * st[3] : 0.f;   // xhat
+          float n = __builtin_fmaf(h[i], gw[i], gb[i]);
+          if constexpr (PER_ROW) n *= gr[i];
+          x[i] = gn_in<V, LANES, WIDE>(i, lane, d.d) ? (__builtin_fmaf(d.res_scale, x[i], n) - st[2]) * st[3] : 0.f;   // xhat
           sw[i] += dy[i] * x[i];
           sb[i] += dy[i];
           dy[i] *= pw[i];
@@ -217,52 +239,79 @@ __global__ __launch_bounds__(256, NE > 16 ? 1 : 2) void gated_norm_bwd_kernel(Ga
         red(s);
         const float m1 = s[0] / d.d, m0 = d.pre == 2 ? s[1] / d.d : 0.f;
 #pragma unroll
-        for (int i = 0; i < NE; i++) t[i] += gn_in<V, LANES>(i, lane, d.d) ? (dy[i] - m0 - x[i] * m1) * st[3] : 0.f;
+        for (int i = 0; i < NE; i++) t[i] += gn_in<V, LANES, WIDE>(i, lane, d.d) ? (dy[i] - m0 - x[i] * m1) * st[3] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < NE; i++) x[i] = t[i] * d.res_scale;   // dx
+      if (on) gn_store<TX, NE, V, LANES, WIDE>(x, (TX*)d.dx + row * d.lddx, lane, d.d);
+      if constexpr (PER_ROW) {
+#pragma unroll
+        for (int i = 0; i < NE; i++) x[i] = t[i] * __builtin_fmaf(h[i], gw[i], gb[i]);   // this row's dgate
+        if (on) gn_store<float, NE, V, LANES, WIDE>(x, d.dgate + row * d.d, lane, d.d);
+#pragma unroll
+        for (int i = 0; i < NE; i++) t[i] *= gr[i];
       }
       float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NE; i++) {
-        x[i] = t[i] * d.res_scale;                 // dx
-        const float tn = t[i] * n[i], u = t[i] * gt[i];
-        n[i] = tn;                                 // this row's dgate
-        sg[i] += tn;
-        qw[i] += u * h[i];
-        qb[i] += u;
-        t[i] = d.post ? u * w[i] : u;
+        sa[i] += t[i] * h[i];
+        sc[i] += t[i];
+        t[i] *= gw[i];
         s[0] += t[i] * h[i];
         s[1] += t[i];
       }
-      if (on) gn_store<TX, NE, V, LANES>(x, (TX*)d.dx + row * d.lddx, lane, d.d);
-      if (on && per_row) gn_store<float, NE, V, LANES>(n, d.dgate + row * d.d, lane, d.d);
       if (d.post) {
         red(s);
         const float m1 = s[0] / d.d, m0 = d.post == 2 ? s[1] / d.d : 0.f;
 #pragma unroll
         for (int i = 0; i < NE; i++) t[i] = (t[i] - m0 - h[i] * m1) * st[1];
       }
-      if (on) gn_store<TH, NE, V, LANES>(t, (TH*)d.dh + row * d.lddh, lane, d.d);
+      if (on) gn_store<TH, NE, V, LANES, WIDE>(t, (TH*)d.dh + row * d.lddh, lane, d.d);
     }
-    // this workgroup's share of gate g: slot (workgroup + gate) is its own (both only ever grow)
-    if (d.gate && !per_row) flush(sg, s0 == g * rpg && s1 == (g + 1) * rpg ? d.dgate + g * d.d : part.base + ((long long)4 * part.C + blockIdx.x + g) * d.d);
+    float w[NE], qw[NE], qb[NE];
+    gn_param<NE, V, LANES, WIDE>(w, gated ? d.gate + g * d.d : nullptr, 1.f, lane, d.d);
+#pragma unroll
+    for (int i = 0; i < NE; i++) { qw[i] = fold[i * 64 * WAVES + tid] + w[i] * sa[i]; qb[i] = fold[(NE + i) * 64 * WAVES + tid] + w[i] * sc[i]; }
+    if (gated) {
+      gn_param<NE, V, LANES, WIDE>(w, d.post_w, 1.f, lane, d.d);
+      gn_param<NE, V, LANES, WIDE>(gb, d.post_b, 0.f, lane, d.d);
+#pragma unroll
+      for (int i = 0; i < NE; i++) sa[i] = w[i] * sa[i] + gb[i] * sc[i];
+      // this workgroup's share of gate g: slot (workgroup + gate) is its own (both only ever grow)
+      flush(sa, s0 == g * rpg && s1 == (g + 1) * rpg ? d.dgate + g * d.d : part.base + ((long long)4 * part.C + blockIdx.x + g) * d.d);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < NE; i++) { fold[i * 64 * WAVES + tid] = qw[i]; fold[(NE + i) * 64 * WAVES + tid] = qb[i]; }   // (read again by the same thread)
     s0 = s1;
   }
+  float qw[NE], qb[NE];
+#pragma unroll
+  for (int i = 0; i < NE; i++) { qw[i] = fold[i * 64 * WAVES + tid]; qb[i] = fold[(NE + i) * 64 * WAVES + tid]; }
   if (d.dpre_w) flush(sw, part.base + (long long)blockIdx.x * d.d);
   if (d.dpre_b) flush(sb, part.base + ((long long)part.C + blockIdx.x) * d.d);
   if (d.dpost_w) flush(qw, part.base + ((long long)2 * part.C + blockIdx.x) * d.d);
   if (d.dpost_b) flush(qb, part.base + ((long long)3 * part.C + blockIdx.x) * d.d);
 }
 
-// sums of the workgroups, in their order: blockIdx.y 0..3 the four parameter vectors, the others the gate rows; 64 columns a block, 4 waves share the workgroups
-__global__ __launch_bounds__(256) void gated_norm_finish_kernel(GatedNormDesc d, GnPart part, long long gates) {
-  __shared__ float fold[4][64];
+// sums of the workgroups, in their order: blockIdx.y 0..3 the four parameter vectors, the others the gate rows; 64 columns a block, 16 waves share the workgroups
+__global__ __launch_bounds__(1024) void gated_norm_finish_kernel(GatedNormDesc d, GnPart part, long long gates) {
+  __shared__ float fold[16][64];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + l;
   auto sum = [&](const float* from, long long lo, long long hi, float* out) {
     float s = 0.f;
-    if (col < d.d)
-      for (long long i = lo + w; i < hi; i += 4) s += from[i * d.d + col];
+    if (col < d.d) {
+#pragma unroll 8
+      for (long long i = lo + w; i < hi; i += 16) s += from[i * d.d + col];
+    }
     fold[w][l] = s;
     __syncthreads();
-    if (w == 0 && col < d.d) out[col] = (fold[0][l] + fold[1][l]) + (fold[2][l] + fold[3][l]);
+    if (w == 0 && col < d.d) {
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) s += fold[i][l];
+      out[col] = s;
+    }
     __syncthreads();
   };
   if (blockIdx.y < 4) {
@@ -277,12 +326,13 @@ __global__ __launch_bounds__(256) void gated_norm_finish_kernel(GatedNormDesc d,
   }
 }
 
-static int gn_teams(int d) { return d <= 1024 ? 4 : d <= 2048 ? 2 : 1; }
+// waves a row
+static int gn_waves(int d) { return d <= 768 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
 static GnPart gn_part(const GatedNormDesc& d, void* ws) {
-  // two workgroups a CU; a run of rows is a whole number of rounds of the workgroup's teams
-  const int teams = gn_teams(d.d);
+  // the workgroups that the chip holds at once (four waves a SIMD, three where a lane has 12 elements); a run of rows is a whole number of the teams' rounds
+  const int k = gn_waves(d.d), teams = k > 4 ? 1 : 4 / k, wgs = k > 4 ? 4096 / k : d.d > 512 && d.d <= 768 ? 768 : 1024;
   GnPart p;
-  p.chunk = (((d.rows + 511) / 512 + teams - 1) / teams) * teams;
+  p.chunk = (((d.rows + wgs - 1) / wgs + teams - 1) / teams) * teams;
   p.C = (int)((d.rows + p.chunk - 1) / p.chunk);
   p.base = (float*)ws;
   return p;
@@ -328,28 +378,32 @@ static int gn_check(const GatedNormDesc& d, int ht, int xt, bool bwd, const char
   return SMBV_OK;
 }
 
-// waves a row and elements a lane by the row's width: as few waves as hold it in 16 registers an operand (32 beyond 4096)
-#define GN_SHAPES(GO)                 \
-  if (d.d <= 512) GO(8, 1)            \
-  else if (d.d <= 1024) GO(16, 1)     \
-  else if (d.d <= 2048) GO(16, 2)     \
-  else if (d.d <= 4096) GO(16, 4)     \
-  else GO(32, 4)
+// elements and their vectors a lane, waves a row
+#define GN_SHAPES(GO)                                                                     \
+  if (d.d <= 512) GO(8, 8, 1)                                                             \
+  else if (d.d <= 768) GO(12, 4, 1)                                                       \
+  else if (d.d <= 1024) GO(8, 8, 2)                                                       \
+  else if (d.d <= 2048) GO(8, 8, 4)                                                       \
+  else if (d.d <= 4096) GO(8, 8, 8)                                                       \
+  else GO(8, 8, 16)
 
 template <class TH, class TX>
 static void gn_fwd(const GatedNormDesc& d, bool wide, hipStream_t st) {
-  const int teams = gn_teams(d.d);
-  const dim3 grid((unsigned)((d.rows + teams - 1) / teams)), blk(256);
-#define GO(NE, K) { if (wide) hipLaunchKernelGGL((gated_norm_fwd_kernel<TH, TX, NE, 8, K>), grid, blk, 0, st, d); \
-                    else hipLaunchKernelGGL((gated_norm_fwd_kernel<TH, TX, NE, 1, K>), grid, blk, 0, st, d); }
+  const int k = gn_waves(d.d), teams = k > 4 ? 1 : 4 / k;
+  const dim3 grid((unsigned)std::min<long long>((d.rows + teams - 1) / teams, 2048)), blk(k > 4 ? 64 * k : 256);   // eight workgroups a CU walk the rows
+#define GO(NE, V, K) { if (wide) hipLaunchKernelGGL((gated_norm_fwd_kernel<TH, TX, NE, V, K, true>), grid, blk, 0, st, d); \
+                       else hipLaunchKernelGGL((gated_norm_fwd_kernel<TH, TX, NE, V, K, false>), grid, blk, 0, st, d); }
   GN_SHAPES(GO)
 #undef GO
 }
 template <class TH, class TX>
 static void gn_bwd(const GatedNormDesc& d, bool wide, const GnPart& part, hipStream_t st) {
-  const dim3 grid(part.C), blk(256);
-#define GO(NE, K) { if (wide) hipLaunchKernelGGL((gated_norm_bwd_kernel<TH, TX, NE, 8, K>), grid, blk, 0, st, d, part); \
-                    else hipLaunchKernelGGL((gated_norm_bwd_kernel<TH, TX, NE, 1, K>), grid, blk, 0, st, d, part); }
+  const int k = gn_waves(d.d);
+  const dim3 grid(part.C), blk(k > 4 ? 64 * k : 256);
+  const bool per_row = d.gate && d.rows_per_gate == 1;
+#define GO1(NE, V, K, W) { if (per_row) hipLaunchKernelGGL((gated_norm_bwd_kernel<TH, TX, NE, V, K, W, true>), grid, blk, 0, st, d, part); \
+                           else hipLaunchKernelGGL((gated_norm_bwd_kernel<TH, TX, NE, V, K, W, false>), grid, blk, 0, st, d, part); }
+#define GO(NE, V, K) { if (wide) GO1(NE, V, K, true) else GO1(NE, V, K, false) }
   GN_SHAPES(GO)
 #undef GO
 }
@@ -375,7 +429,7 @@ int gated_norm_bwd(const GatedNormDesc& d, int ht, int xt, void* ws, size_t ws_b
   const GnPart part = gn_part(d, ws);
   GN_TYPES(gn_bwd, d, wide, part, st)
   const long long gates = gn_gates(d);
-  hipLaunchKernelGGL(gated_norm_finish_kernel, dim3((d.d + 63) / 64, 4 + (unsigned)std::min<long long>(gates, 512)), dim3(256), 0, st, d, part, gates);
+  hipLaunchKernelGGL(gated_norm_finish_kernel, dim3((d.d + 63) / 64, 4 + (unsigned)std::min<long long>(gates, 512)), dim3(1024), 0, st, d, part, gates);
   return check_launch("gated_norm_bwd");
 }
 
