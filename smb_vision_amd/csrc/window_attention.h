@@ -260,6 +260,14 @@ struct WinCopy {
 // Left alone the compiler puts an LDS read right in front of the product that waits for it.  Code on the two sides of this line stays there: operands are read
 // on one side and used on the other, where the next ones are read.
 #define WIN_AHEAD() __builtin_amdgcn_sched_barrier(0)
+// The basic block's products and vector instructions in turn: N times one and V
+template <int N, int V> __device__ __forceinline__ void win_weave() {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+  }
+}
 
 // x of this lane and of lane l ^ 32
 __device__ __forceinline__ void win_halves(float x, float& u, float& v) {

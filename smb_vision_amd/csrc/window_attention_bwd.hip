@@ -202,19 +202,23 @@ __device__ __forceinline__ WinRun win_key_rows(const WinDesc& d, const WinSeq& s
 // rows are, 320 tiles of rows against 66 at 20,480 tokens and a window of 4097.  So their rows go to c1 workgroups, the other tiles' to c2 (1 unless there are too
 // few tiles to fill the chip); a tile's workgroups leave their fp32 sums in the workspace and a second launch adds them in order.
 struct WinSplit {
-  int tiles, nsink, c1, c2, units, roles;  // units: workgroups of one key head; roles: 2 when dK and dV have workgroups of their own
-  float* part;                             // [B, Hk][slots][dK | dV][BK keys][DP]
+  int tiles, nsink, c1, c2, units;  // units: workgroups of one key head
+  float* part;                      // [B, Hk][slots][dK | dV][BK keys][DP]
 };
 __device__ __host__ __forceinline__ int win_split_slots(const WinSplit& s) { return (s.c1 > 1 ? s.nsink * s.c1 : 0) + (s.c2 > 1 ? (s.tiles - s.nsink) * s.c2 : 0); }
 
-// PART: 1 dV (products S, dV), 2 dK (S, dP, dK), 3 both
-template <class E, int DP, int NW, int NS, int PART>
-__device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wrows, const WinSplit& sp, unsigned char* smem, int unit, int hk, int b) {
+// Heads wider than 64 keep 192 registers of accumulators and of K and V: one wave a SIMD with all the registers, reading its operands ahead of their products,
+// beats both two waves that spill (1164 us against 696 at 4 x 4093 tokens, 16 heads on 4 of 128) and workgroups of their own for dK and dV, which form S twice.
+template <class E, int DP, int NW, int NS>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 ? 1 : 2, DP == 128 ? 1 : 2))) void win_dkv_kernel(WinDesc d, WinRows wrows, WinSplit sp) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BK = 32 * NW, SLOT = 2 * IMG, STAT = NS * SLOT;   // STAT: where the rows' numbers lie
-  constexpr bool HAS_V = PART & 1, HAS_K = PART & 2, AHEAD = DP == 128;   // see the forward
+  constexpr bool AHEAD = DP == 128;   // see the forward
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NS * (SLOT + 4 * 256)];   // slots of Q | dO, then of LSE | delta | exponent | spare
   using v8 = typename E::v8;
   using Copy = WinCopy<DP, NW>;
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), r31 = l & 31, h2 = l >> 5;
+  int unit, hk, b;
+  win_block_order(sp.units, d.Hk, d.B, unit, hk, b);
   const bool sink = unit < sp.nsink * sp.c1;
   const int c12 = sink ? sp.c1 : sp.c2, rest = sink ? unit : unit - sp.nsink * sp.c1, tile = (sink ? 0 : sp.nsink) + rest / c12, share = rest % c12;
   const WinSeq seq = win_seq(d, b);
@@ -239,7 +243,7 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
     const int ch = 16 * ks + 8 * h2;
     if (key < seq.klen && ch < d.D) {
       x = *(const u32x4*)(d.k + b * d.sk.b + key * d.sk.r + hk * d.sk.h + ch);
-      if constexpr (HAS_K) y = *(const u32x4*)(d.v + b * d.sv.b + key * d.sv.r + hk * d.sv.h + ch);
+      y = *(const u32x4*)(d.v + b * d.sv.b + key * d.sv.r + hk * d.sv.h + ch);
     }
     asm volatile("" : "+v"(x), "+v"(y));
     kf[ks] = __builtin_bit_cast(v8, x);
@@ -299,7 +303,7 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
     if (kw0 > klast || q0 + 64 <= first.lo || q0 >= any_hi) return;   // nobody sees these keys
     const bool all = q0 >= all_lo && q0 + 64 <= all_hi;
     float unit = 1.f;
-    if constexpr (E::half && HAS_K) {
+    if constexpr (E::half) {
       int e = *(const int*)(st + 512 + 4 * l);
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 64));
@@ -313,80 +317,85 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
       }
       unit = emax == WIN_NO_EXP ? 1.f : ldexpf(1.f, -emax);
     }
+    // 32 rows at a time: qt's products over the channels, its P and dS, its products over the rows.  The matrix pipe runs beside the vector unit when their
+    // instructions alternate (8 products and 64 others: 173 us together, 125 and 115 alone), so each half's vector work stands next to the other's products.
+    f32x16 s[2], dp[2];
+    u32x4 qa[2][KS], ga[2][KS];
+    v8 pf[2][2], ds[2][2];
+    s16x8 gc[2][2][DT], qc[2][2][DT];
+    auto rows = [&](int qt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int qt = 0; qt < 2; qt++) {
-      f32x16 s, dp;
+      for (int ks = 0; ks < KS; ks++) { qa[qt][ks] = rd.rows(ks, off + 64 * DP * qt); ga[qt][ks] = rd.rows(ks, off + IMG + 64 * DP * qt); }
 #pragma unroll
-      for (int x = 0; x < 16; x++) s[x] = 0.f;
-      if constexpr (HAS_K) {
+      for (int x = 0; x < 4; x++) {
+        const f32x4 de = *(const f32x4*)(st + 256 + (32 * qt + 8 * x + 4 * h2) * 4);
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-          const f32x4 de = *(const f32x4*)(st + 256 + (32 * qt + 8 * x + 4 * h2) * 4);
-#pragma unroll
-          for (int y = 0; y < 4; y++) dp[4 * x + y] = de[y];
-        }
+        for (int y = 0; y < 4; y++) { s[qt][4 * x + y] = 0.f; dp[qt][4 * x + y] = de[y]; }
       }
-      u32x4 qa[KS], ga[KS];
-      auto read = [&](int ks) __attribute__((always_inline)) {
-        qa[ks] = rd.rows(ks, off + 64 * DP * qt);
-        if constexpr (HAS_K) ga[ks] = rd.rows(ks, off + IMG + 64 * DP * qt);
-      };
-      read(0);
-      read(1);
+    };
+    auto scores = [&](int qt) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ks += 2) {   // two 16-channel steps ahead
-        if constexpr (AHEAD) WIN_AHEAD();
-        if (ks + 2 < KS) { read(ks + 2); read(ks + 3); }
-#pragma unroll
-        for (int y = ks; y < ks + 2; y++) {
-          s = E::mfma(__builtin_bit_cast(v8, qa[y]), kf[y], s);
-          if constexpr (HAS_K) dp = E::mfma(__builtin_bit_cast(v8, ga[y]), vf[y], dp);
-        }
+      for (int ks = 0; ks < KS; ks++) {
+        s[qt] = E::mfma(__builtin_bit_cast(v8, qa[qt][ks]), kf[ks], s[qt]);
+        dp[qt] = E::mfma(__builtin_bit_cast(v8, ga[qt][ks]), vf[ks], dp[qt]);
       }
-      if (!all) {
-        const int o = q0 + 32 * qt + 4 * h2, lo = mine.lo - o, hi = min(mine.hi, rhi) - o;
+    };
+    auto mask = [&](int qt) __attribute__((always_inline)) {
+      const int o = q0 + 32 * qt + 4 * h2, lo = mine.lo - o, hi = min(mine.hi, rhi) - o;
 #pragma unroll
-        for (int x = 0; x < 16; x++) {
-          const int r = (x & 3) + 8 * (x >> 2);
-          const bool vis = r >= lo && r < hi;
-          s[x] = vis ? s[x] : -INFINITY;
-          if constexpr (HAS_K) dp[x] = vis ? dp[x] : 0.f;
-        }
+      for (int x = 0; x < 16; x++) {
+        const int r = (x & 3) + 8 * (x >> 2);
+        const bool vis = r >= lo && r < hi;
+        s[qt][x] = vis ? s[qt][x] : -INFINITY;
+        dp[qt][x] = vis ? dp[qt][x] : 0.f;
       }
-      f32x4 ls[4];
+    };
+    auto cols = [&](int qt) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < 4; x++) ls[x] = *(const f32x4*)(st + (32 * qt + 8 * x + 4 * h2) * 4);
-      s16x8 gc[2][DT], qc[2][DT];
-      auto cols = [&](int half) __attribute__((always_inline)) {
+      for (int half = 0; half < 2; half++)
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
-          if constexpr (HAS_V) gc[half][dt] = rd.cols(dt, off + IMG + 64 * DP * qt + 32 * DP * half);
-          if constexpr (HAS_K) qc[half][dt] = rd.cols(dt, off + 64 * DP * qt + 32 * DP * half);
+          gc[qt][half][dt] = rd.cols(dt, off + IMG + 64 * DP * qt + 32 * DP * half);
+          qc[qt][half][dt] = rd.cols(dt, off + 64 * DP * qt + 32 * DP * half);
         }
-      };
-      cols(0);
-      if constexpr (AHEAD) WIN_AHEAD();
+    };
+    auto probs = [&](int qt) __attribute__((always_inline)) {
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        v8 pf, ds;
+      for (int x = 0; x < 16; x++) {
+        const f32x4 ls = *(const f32x4*)(st + (32 * qt + 8 * (x >> 2) + 4 * h2) * 4);
+        const float p = fast_exp2(__builtin_fmaf(s[qt][x], c, -ls[x & 3]));
+        float g = p * dp[qt][x];
+        if constexpr (E::half) g *= unit;
+        pf[qt][x >> 3][x & 7] = (typename E::e)p;
+        ds[qt][x >> 3][x & 7] = (typename E::e)g;
+      }
+      asm volatile("" : "+v"(pf[qt][0]), "+v"(pf[qt][1]), "+v"(ds[qt][0]), "+v"(ds[qt][1]));   // (here, not where they are first used)
+    };
+    auto grads = [&](int qt) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const float p = fast_exp2(__builtin_fmaf(s[8 * half + x], c, -ls[2 * half + (x >> 2)][x & 3]));
-          if constexpr (HAS_V) pf[x] = (typename E::e)p;
-          if constexpr (HAS_K) {
-            float g = p * dp[8 * half + x];
-            if constexpr (E::half) g *= unit;
-            ds[x] = (typename E::e)g;
-          }
-        }
-        if (half == 0) cols(1);
+      for (int half = 0; half < 2; half++)
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
-          if constexpr (HAS_V) dv[dt] = E::mfma(__builtin_bit_cast(v8, gc[half][dt]), pf, dv[dt]);
-          if constexpr (HAS_K) dk[dt] = E::mfma(__builtin_bit_cast(v8, qc[half][dt]), ds, dk[dt]);
+          dv[dt] = E::mfma(__builtin_bit_cast(v8, gc[qt][half][dt]), pf[qt][half], dv[dt]);
+          dk[dt] = E::mfma(__builtin_bit_cast(v8, qc[qt][half][dt]), ds[qt][half], dk[dt]);
         }
-      }
-    }
+    };
+    constexpr int VALU = E::half ? 72 : 56;   // of probs
+    rows(0);
+    if constexpr (AHEAD) WIN_AHEAD();
+    rows(1);
+    scores(0);
+    if (!all) mask(0);
+    cols(0);
+    scores(1);
+    probs(0);
+    win_weave<2 * KS, VALU / (2 * KS)>();
+    if (!all) mask(1);
+    cols(1);
+    grads(0);
+    probs(1);
+    win_weave<4 * DT, VALU / (4 * DT)>();
+    grads(1);
   };
   if (rlo < rhi) win_walk<NS, SLOT>((rhi - rlo + 63) / 64, win_arrived<(NS - 2) * (2 * Copy::NP + 1)>, stage, rowtile, [&](int by) { rd.move(by); });
   const float f = E::half && emax != WIN_NO_EXP ? ldexpf(d.scale, emax) : d.scale;
@@ -398,8 +407,8 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
 #pragma unroll
       for (int rg = 0; rg < 4; rg++) {
         float* at = part + (dt * BK + 32 * w + r31) * 32 + 8 * rg + 4 * h2;
-        if constexpr (HAS_K) *(f32x4*)at = (f32x4){dk[dt][4 * rg] * f, dk[dt][4 * rg + 1] * f, dk[dt][4 * rg + 2] * f, dk[dt][4 * rg + 3] * f};
-        if constexpr (HAS_V) *(f32x4*)(at + BK * DP) = (f32x4){dv[dt][4 * rg], dv[dt][4 * rg + 1], dv[dt][4 * rg + 2], dv[dt][4 * rg + 3]};
+        *(f32x4*)at = (f32x4){dk[dt][4 * rg] * f, dk[dt][4 * rg + 1] * f, dk[dt][4 * rg + 2] * f, dk[dt][4 * rg + 3] * f};
+        *(f32x4*)(at + BK * DP) = (f32x4){dv[dt][4 * rg], dv[dt][4 * rg + 1], dv[dt][4 * rg + 2], dv[dt][4 * rg + 3]};
       }
     return;
   }
@@ -416,21 +425,9 @@ __device__ __forceinline__ void win_dkv_body(const WinDesc& d, const WinRows& wr
       float a[4], g[4];
 #pragma unroll
       for (int x = 0; x < 4; x++) { a[x] = live ? dk[dt][4 * rg + x] * f : 0.f; g[x] = live ? dv[dt][4 * rg + x] : 0.f; }
-      if constexpr (HAS_K) *(u32x2*)(ok + d0) = (u32x2){el_pack<E>(a[0], a[1]), el_pack<E>(a[2], a[3])};
-      if constexpr (HAS_V) *(u32x2*)(ov + d0) = (u32x2){el_pack<E>(g[0], g[1]), el_pack<E>(g[2], g[3])};
+      *(u32x2*)(ok + d0) = (u32x2){el_pack<E>(a[0], a[1]), el_pack<E>(a[2], a[3])};
+      *(u32x2*)(ov + d0) = (u32x2){el_pack<E>(g[0], g[1]), el_pack<E>(g[2], g[3])};
     }
-}
-
-// ROLES 2 (heads wider than 64): dK and dV in 128 accumulator registers beside K and V do not leave room for two waves a SIMD; workgroups of their own do, at the
-// price of a second S (5 products instead of 4).  The longer dK workgroups of a key head come first.
-template <class E, int DP, int NW, int NS, int ROLES>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void win_dkv_kernel(WinDesc d, WinRows wrows, WinSplit sp) {
-  __shared__ __attribute__((aligned(16))) unsigned char smem[NS * (4 * 64 * DP + 4 * 256)];   // slots of Q | dO | LSE | delta | exponent | spare
-  int unit, hk, b;
-  win_block_order(sp.units * ROLES, d.Hk, d.B, unit, hk, b);
-  if constexpr (ROLES == 1) win_dkv_body<E, DP, NW, NS, 3>(d, wrows, sp, smem, unit, hk, b);
-  else if (unit < sp.units) win_dkv_body<E, DP, NW, NS, 2>(d, wrows, sp, smem, unit, hk, b);
-  else win_dkv_body<E, DP, NW, NS, 1>(d, wrows, sp, smem, unit - sp.units, hk, b);
 }
 
 // adds the shares of the tiles that were split: a workgroup takes 1024 / DP keys of one tile's dK or dV
@@ -464,16 +461,15 @@ static int win_dp(const WinDesc& d) { return d.D <= 32 ? 32 : d.D <= 64 ? 64 : 1
 static WinSplit win_split(const WinDesc& d) {
   WinSplit s = {};
   const int bk = WIN_BK;
-  s.roles = d.D > 64 ? 2 : 1;
   s.tiles = (d.Sk + bk - 1) / bk;
   s.nsink = d.left < 0 ? 0 : std::min(s.tiles, (int)(((long long)std::min(d.sinks, d.Sk) + bk - 1) / bk));
   // rows that see a tile: all (a sink, an open window to the left), or those of a window
   const long long all = (long long)d.Sq * d.G, window = d.left < 0 || d.right < 0 ? all : std::min<long long>(all, ((long long)d.left + d.right + bk) * d.G);
-  const long long plain = (long long)(s.tiles - s.nsink) * d.Hk * d.B * s.roles;
+  const long long plain = (long long)(s.tiles - s.nsink) * d.Hk * d.B;
   // A share costs its sums' way through memory (128 KiB at 128 keys of 128 channels, out and back) and saves a part of its tile's rows, a microsecond or two for
   // 64 of them: no share has less than 1024 rows, and tiles are split only as far as there is room for more workgroups (two a CU; the sinks' four)
   s.c2 = (int)std::max<long long>(1, std::min<long long>({512 / std::max<long long>(plain, 1), window / 1024, 64}));
-  const long long share = std::max<long long>(1024, (window + s.c2 - 1) / s.c2), sinks = (long long)s.nsink * d.Hk * d.B * s.roles;
+  const long long share = std::max<long long>(1024, (window + s.c2 - 1) / s.c2), sinks = (long long)s.nsink * d.Hk * d.B;
   s.c1 = (int)std::max<long long>(1, std::min<long long>({(all + share - 1) / share, 1024 / std::max<long long>(sinks, 1), 64}));
   if (s.nsink == s.tiles) s.c2 = 1;
   if (s.nsink == 0) s.c1 = 1;
@@ -511,16 +507,16 @@ static int win_bwd(const WinDesc& d, void* ws, hipStream_t st) {
   if (d.Sk > 0) {
     WinSplit sp = win_split(d);
     sp.part = (float*)((char*)ws + nb * (E::half ? 3 : 2));
-    const dim3 grid((unsigned)(heads * sp.units * sp.roles));
+    const dim3 grid((unsigned)(heads * sp.units));
     const int ntile = (sp.c1 > 1 ? sp.nsink : 0) + (sp.c2 > 1 ? sp.tiles - sp.nsink : 0);
-#define GO(DP, NW, NS, ROLES)                                                                                                                          \
+#define GO(DP, NW, NS)                                                                                                                          \
   {                                                                                                                                                    \
-    hipLaunchKernelGGL((win_dkv_kernel<E, DP, NW, NS, ROLES>), grid, dim3(64 * NW), 0, st, d, wr, sp);                                                \
+    hipLaunchKernelGGL((win_dkv_kernel<E, DP, NW, NS>), grid, dim3(64 * NW), 0, st, d, wr, sp);                                                \
     if (ntile) hipLaunchKernelGGL((win_dkv_join_kernel<E, DP, 32 * NW>), dim3((unsigned)(2 * (32 * NW / (1024 / DP)) * ntile * heads)), dim3(256), 0, st, d, sp); \
   }
-    if (d.D <= 32) GO(32, 4, 4, 1)
-    else if (d.D <= 64) GO(64, 4, 4, 1)
-    else GO(128, 4, 2, 2)
+    if (d.D <= 32) GO(32, 4, 4)
+    else if (d.D <= 64) GO(64, 4, 4)
+    else GO(128, 4, 4)
 #undef GO
   }
   return check_launch("window_attention_bwd");
