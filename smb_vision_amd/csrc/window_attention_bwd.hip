@@ -60,7 +60,6 @@ __global__ __launch_bounds__(256) void win_rows_kernel(WinDesc d, WinRows wr) {
 template <class E, int DP, int NW, int NS, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void win_dq_kernel(WinDesc d, WinRows wrows) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BM = 32 * NW;
-  constexpr bool AHEAD = DP == 128;   // see the forward
   using v8 = typename E::v8;
   using Copy = WinCopy<DP, NW>;
   __shared__ __attribute__((aligned(16))) unsigned char smem[NS * 2 * IMG];
@@ -134,40 +133,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
       f32x16 s, dp;
 #pragma unroll
       for (int x = 0; x < 16; x++) s[x] = 0.f;
-      dp = cdel;
-      u32x4 kf[KS], vf[KS];
-      auto read = [&](int ks) __attribute__((always_inline)) {
-        kf[ks] = rd.rows(ks, off + 64 * DP * kt);
-        vf[ks] = rd.rows(ks, off + IMG + 64 * DP * kt);
-      };
-      read(0);
-      read(1);
 #pragma unroll
-      for (int ks = 0; ks < KS; ks += 2) {   // two 16-channel steps ahead
-        if constexpr (AHEAD) WIN_AHEAD();
-        if (ks + 2 < KS) { read(ks + 2); read(ks + 3); }
-#pragma unroll
-        for (int y = ks; y < ks + 2; y++) {
-          s = E::mfma(__builtin_bit_cast(v8, kf[y]), qf[y], s);
-          dp = E::mfma(__builtin_bit_cast(v8, vf[y]), gf[y], dp);
-        }
+      for (int ks = 0; ks < KS; ks++) {
+        s = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + 64 * DP * kt)), qf[ks], s);
+        dp = E::mfma(__builtin_bit_cast(v8, rd.rows(ks, off + IMG + 64 * DP * kt)), gf[ks], ks == 0 ? cdel : dp);
       }
       if (kind != WIN_ALL) win_mask(s, kind, view, 64 * j + 32 * kt + 4 * h2);   // (its exp2 is 0, and dP is finite as far as dO and V are)
-      s16x8 kc[2][DT];
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++) kc[0][dt] = rd.cols(dt, off + 64 * DP * kt);
-      if constexpr (AHEAD) WIN_AHEAD();
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         v8 ds;
 #pragma unroll
         for (int x = 0; x < 8; x++) ds[x] = (typename E::e)(fast_exp2(__builtin_fmaf(s[8 * half + x], c, -lse2)) * dp[8 * half + x]);
-        if (half == 0) {
 #pragma unroll
-          for (int dt = 0; dt < DT; dt++) kc[1][dt] = rd.cols(dt, off + 64 * DP * kt + 32 * DP);
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) acc[dt] = E::mfma(__builtin_bit_cast(v8, kc[half][dt]), ds, acc[dt]);
+        for (int dt = 0; dt < DT; dt++) acc[dt] = E::mfma(__builtin_bit_cast(v8, rd.cols(dt, off + 64 * DP * kt + 32 * DP * half)), ds, acc[dt]);
       }
     }
   };
