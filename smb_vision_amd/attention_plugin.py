@@ -13,12 +13,19 @@ softmax(QK^T * scaling) V and everything else in PyTorch.  This is the operator-
 (modeling_videomae.py / modeling_vjepa.py) is the shipped path and avoids the head-major <-> token-major copies this interface forces.
 
 No fallback: anything the kernels do not compute (masks, dropout, causal, head widths other than 64 / 32, no GPU) raises.
+
+`register_window()` adds "smbv_window": smbv_window_attention_fwd / _bwd under the same interface - a sliding window (bound at registration, or the model's own
+`sliding_window`), first tokens that stay visible, causal models, grouped key heads, queries at the end of a longer cache, bf16 and fp16, head widths that are
+multiples of 8 up to 128 - and without copies, since those kernels take the head-major strides as they are.
 """
+import functools
+
 import torch
 
 from . import ops
 
 NAME = "smbv"
+WINDOW_NAME = "smbv_window"
 
 
 class _SmbvAttentionFn(torch.autograd.Function):
@@ -71,4 +78,86 @@ def register(name=NAME):
     """Make `config._attn_implementation = name` select the MI355X kernels (transformers.AttentionInterface)."""
     from transformers import AttentionInterface
     AttentionInterface.register(name, smbv_attention)
+    return name
+
+
+def _not_captured():
+    # (autograd's own nodes of a leaf stay on the stream that first used them: a backward pass captured while an eager graph of the same leaves lives ends the
+    # process.  ops.window_attention_fwd / _bwd are what a captured training step calls.)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("smbv window attention: training through autograd cannot be captured into a graph; capture ops.window_attention_fwd / _bwd instead")
+
+
+class _SmbvWindowAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kw):
+        _not_captured()
+        out, lse, out_lo = ops.window_attention_fwd(q, k, v, resid=True, **kw)
+        ctx.save_for_backward(q, k, v, out, lse, out_lo)
+        ctx.kw = kw
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        _not_captured()
+        q, k, v, out, lse, out_lo = ctx.saved_tensors
+        return (*ops.window_attention_bwd(q, k, v, out, _rows_of_heads(d_out.to(q.dtype)), lse, o_lo=out_lo, **ctx.kw), None)
+
+
+def _rows_of_heads(t):
+    """t [B, S, H, D] as the kernels can read it: contiguous channels, 16-byte steps."""
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3)):
+        return t.contiguous()
+    return t
+
+
+def smbv_window_attention(module, query, key, value, attention_mask=None, *, scaling=None, dropout=0.0, is_causal=None, sliding_window=None, sinks=0, **kwargs):
+    """transformers attention-interface function for query [B, H, Sq, D], key / value [B, Hk, Sk, D]; returns (context [B, Sq, H, D] in the dtype of query, None).
+
+    sliding_window: None, or W - keys closer than W positions, in both directions unless the attention is causal -, or (left, right) - as many keys to either
+    side, -1 for all.  is_causal: None takes the module's own `is_causal` (False if it has none).  The queries are the last Sq of the Sk positions, all of which
+    hold tokens: no preallocated cache with empty slots.  sinks: first keys that stay visible to every later query.  fp32 operands are rounded to bf16."""
+    if attention_mask is not None:
+        raise ValueError("smbv window attention: masks are not supported (the window, causality and the first tokens are arguments)")
+    if dropout:
+        raise ValueError("smbv window attention: attention dropout is not supported")
+    if query.dim() != 4 or key.dim() != 4 or key.shape != value.shape or key.shape[0] != query.shape[0] or key.shape[3] != query.shape[3] or query.shape[1] % max(key.shape[1], 1):
+        raise ValueError(f"smbv window attention: expected query [B, H, Sq, D] and key, value [B, Hk, Sk, D] with H a multiple of Hk, got {tuple(query.shape)}, "
+                         f"{tuple(key.shape)}, {tuple(value.shape)}")
+    if query.shape[3] % 8 or not 0 < query.shape[3] <= 128:
+        raise ValueError(f"smbv window attention: head width {query.shape[3]} (a multiple of 8 up to 128)")
+    if not query.is_cuda:
+        raise RuntimeError("smbv window attention needs an MI355X: there is no CPU path")
+    causal = bool(getattr(module, "is_causal", False) if is_causal is None else is_causal)
+    if sliding_window is None:
+        left = right = -1
+    elif isinstance(sliding_window, int):
+        if sliding_window < 1:
+            raise ValueError(f"smbv window attention: sliding_window {sliding_window}")
+        left = right = sliding_window - 1
+    else:
+        left, right = (int(x) for x in sliding_window)
+    if causal:
+        right = 0
+    dtype = query.dtype if query.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+    q, k, v = (_rows_of_heads(t.transpose(1, 2).to(dtype)) for t in (query, key, value))
+    kw = dict(left=left, right=right, sinks=int(sinks), scale=None if scaling is None else float(scaling))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out = _SmbvWindowAttentionFn.apply(q, k, v, kw)
+    else:
+        out = ops.window_attention_fwd(q, k, v, **kw)[0]
+    return out.to(query.dtype), None
+
+
+def register_window(name=WINDOW_NAME, *, window=None, sinks=0):
+    """Make `config._attn_implementation = name` select the windowed kernels.  window: what takes the place of `sliding_window` in models that pass none (the
+    reference's encoders among them); sinks: first tokens that stay visible."""
+    from transformers import AttentionInterface
+
+    @functools.wraps(smbv_window_attention)
+    def attend(module, query, key, value, attention_mask=None, *, sliding_window=None, **kwargs):
+        return smbv_window_attention(module, query, key, value, attention_mask, sliding_window=window if sliding_window is None else sliding_window, sinks=sinks, **kwargs)
+
+    AttentionInterface.register(name, attend)
     return name

@@ -231,3 +231,15 @@ def test_gated_norm_more_arguments(dry):
         ops.gated_norm_bwd(dx1, dy, h, x, st, out=(h, x.clone()), **a)
     with pytest.raises(ValueError):
         ops.gated_norm_bwd(None, dy, h, x, st, **{**a, "pre": None, "pre_w": None, "pre_b": None})
+
+
+def test_window_plugin_registers_and_refuses_cpu():
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+    from smb_vision_amd import attention_plugin
+    name = attention_plugin.register_window(window=(8, 8), sinks=2)
+    assert name == "smbv_window" and name in ALL_ATTENTION_FUNCTIONS
+    q = Z(1, 2, 16, 64)
+    with pytest.raises(RuntimeError):
+        ALL_ATTENTION_FUNCTIONS[name](torch.nn.Module(), q, q, q, None, scaling=0.125, dropout=0.0)
+    with pytest.raises(ValueError):
+        ALL_ATTENTION_FUNCTIONS[name](torch.nn.Module(), q, q, q, Z(1, 1, 16, 16))
