@@ -22,7 +22,8 @@ template <> struct RopeIo<__bf16> {
 };
 template <> struct RopeIo<_Float16> {
   static __device__ __forceinline__ float ld(_Float16 x) { return (float)x; }
-  static __device__ __forceinline__ _Float16 st(float x) { return (_Float16)x; }
+  // (kept apart from the sum in front of it: v_fma_mixlo_f16 rounds the two at once, and some of a variant's elements would have it and others not)
+  static __device__ __forceinline__ _Float16 st(float x) { asm("" : "+v"(x)); return (_Float16)x; }
 };
 template <class T, int V> struct __attribute__((aligned(V > 2 ? sizeof(T) * V : sizeof(T)))) RopeVec { T e[V]; };  // (V = 2: the fallback for any alignment)
 
@@ -97,6 +98,7 @@ static int rope_axes_t(const RopeAxesDesc& d, hipStream_t st) {
   const long long n = (long long)d.B * d.S;
   // enough blocks to fill the chip, at most ROPE_LDS_PAIRS angles a block
   const int tpb = (int)std::max<long long>(1, std::min<long long>(ROPE_LDS_PAIRS / d.P, n / 2048));
+  if (n / tpb >= (1 << 24) - 1) { set_error("rope_axes: %d x %d tokens are too many for one call", d.B, d.S); return SMBV_ERR_SHAPE; }   // (a launch ends at 2^32 threads)
   const dim3 grid((unsigned)((n + tpb - 1) / tpb)), blk(256);
   long long bits = (d.H ? ((uintptr_t)d.q | (uintptr_t)d.qo) / sizeof(T) | d.sq[0] | d.sq[1] | d.sq[2] | d.sqo[0] | d.sqo[1] | d.sqo[2] : 0) |
                    (d.Hk ? ((uintptr_t)d.k | (uintptr_t)d.ko) / sizeof(T) | d.sk[0] | d.sk[1] | d.sk[2] | d.sko[0] | d.sko[1] | d.sko[2] : 0) |

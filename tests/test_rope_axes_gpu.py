@@ -92,6 +92,18 @@ def test_views_in_place_and_alignment(ops, dtype, interleaved):
     assert torch.equal(out[:, :S, :H], want[0]) and bool((out[:, S:] == 7).all()) and bool((out[:, :, H] == 7).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_every_alignment_rounds_alike(ops, dtype, interleaved):
+    """262,144 elements through the vector kernel and, one element further on, through the one for any alignment."""
+    g = torch.Generator().manual_seed(7)
+    q = torch.randn(4, 512, 2, 64, generator=g).to(dtype).cuda()
+    pos, inv = torch.randint(0, 5000, (2, 4, 512), dtype=torch.int32, generator=g).cuda(), torch.rand(32, generator=g).cuda()
+    odd = torch.empty(q.numel() + 1, dtype=dtype, device="cuda")[1:].view_as(q).copy_(q)
+    want = ops.rope_axes(q, None, pos, inv, (12, 20), interleaved=interleaved)[0]
+    assert torch.equal(want, ops.rope_axes(odd, None, pos, inv, (12, 20), interleaved=interleaved)[0])
+
+
 def test_captured_and_empty(ops):
     q, k = torch.randn(2, 9, 2, 64, device="cuda"), torch.randn(2, 9, 1, 64, device="cuda")
     pos = torch.arange(9, dtype=torch.int32, device="cuda").repeat(2, 2, 1)
