@@ -165,7 +165,8 @@ __global__ __launch_bounds__(K > 4 ? 64 * K : 256) void gated_norm_fwd_kernel(Ga
   }
 }
 
-// workspace of the backward: sums of C workgroups, [C][d] each: pre_w | pre_b | post_w | post_b, then the gate's, [C + gates][d]
+// workspace of the backward: sums of C workgroups, [C][d] each: pre_w | pre_b | post_w | post_b, then [C][2][d]: of the gates that a workgroup shares with others -
+// the one that its rows begin with, and the one that begins inside them and goes on behind them
 struct GnPart { float* base; int C; long long chunk; };
 
 template <class TH, class TX, int NE, int V, int K, bool WIDE, bool PER_ROW>
@@ -277,8 +278,7 @@ __global__ __launch_bounds__(K > 4 ? 64 * K : 256) __attribute__((amdgpu_waves_p
       gn_param<NE, V, LANES, WIDE>(gb, d.post_b, 0.f, lane, d.d);
 #pragma unroll
       for (int i = 0; i < NE; i++) sa[i] = w[i] * sa[i] + gb[i] * sc[i];
-      // this workgroup's share of gate g: slot (workgroup + gate) is its own (both only ever grow)
-      flush(sa, s0 == g * rpg && s1 == (g + 1) * rpg ? d.dgate + g * d.d : part.base + ((long long)4 * part.C + blockIdx.x + g) * d.d);
+      flush(sa, s0 == g * rpg && s1 == (g + 1) * rpg ? d.dgate + g * d.d : part.base + ((long long)4 * part.C + 2 * blockIdx.x + (s0 == c0 ? 0 : 1)) * d.d);
       __syncthreads();
     }
 #pragma unroll
@@ -298,11 +298,12 @@ __global__ __launch_bounds__(K > 4 ? 64 * K : 256) __attribute__((amdgpu_waves_p
 __global__ __launch_bounds__(1024) void gated_norm_finish_kernel(GatedNormDesc d, GnPart part, long long gates) {
   __shared__ float fold[16][64];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + l;
-  auto sum = [&](const float* from, long long lo, long long hi, float* out) {
+  // rows `step` apart of the workgroups [lo, hi), the first one's `first` further on
+  auto sum = [&](const float* from, int step, int first, long long lo, long long hi, float* out) {
     float s = 0.f;
     if (col < d.d) {
 #pragma unroll 8
-      for (long long i = lo + w; i < hi; i += 16) s += from[i * d.d + col];
+      for (long long i = lo + w; i < hi; i += 16) s += from[(i * step + (i == lo ? first : 0)) * d.d + col];
     }
     fold[w][l] = s;
     __syncthreads();
@@ -316,13 +317,13 @@ __global__ __launch_bounds__(1024) void gated_norm_finish_kernel(GatedNormDesc d
   };
   if (blockIdx.y < 4) {
     float* out = blockIdx.y == 0 ? d.dpre_w : blockIdx.y == 1 ? d.dpre_b : blockIdx.y == 2 ? d.dpost_w : d.dpost_b;
-    if (out) sum(part.base + (long long)blockIdx.y * part.C * d.d, 0, part.C, out);
+    if (out) sum(part.base + (long long)blockIdx.y * part.C * d.d, 1, 0, 0, part.C, out);
     return;
   }
   for (long long g = blockIdx.y - 4; g < gates; g += gridDim.y - 4) {
     const long long r0 = g * d.rows_per_gate, r1 = r0 + d.rows_per_gate, lo = r0 / part.chunk, hi = (r1 - 1) / part.chunk + 1;
     // (one workgroup that held all of a gate's rows has written the sum itself)
-    if (hi - lo > 1) sum(part.base + ((long long)4 * part.C + g) * d.d, lo, hi, d.dgate + g * d.d);
+    if (hi - lo > 1) sum(part.base + (long long)4 * part.C * d.d, 2, r0 == lo * part.chunk ? 0 : 1, lo, hi, d.dgate + g * d.d);
   }
 }
 
@@ -342,7 +343,7 @@ static long long gn_gates(const GatedNormDesc& d) { return d.gate && d.rows_per_
 size_t gated_norm_bwd_workspace_bytes(const GatedNormDesc& d) {
   if (d.rows <= 0 || d.d <= 0) return 256;
   const GnPart p = gn_part(d, nullptr);
-  return ((size_t)5 * p.C + gn_gates(d)) * d.d * sizeof(float) + 256;
+  return (size_t)(gn_gates(d) ? 6 : 4) * p.C * d.d * sizeof(float) + 256;
 }
 
 static int gn_check(const GatedNormDesc& d, int ht, int xt, bool bwd, const char* what, bool& wide) {
