@@ -185,8 +185,6 @@ __device__ __forceinline__ void win_block_order(int nt, int Hk, int B, int& tile
   hk = hb % Hk;
   b = hb / Hk;
 }
-// row of register i of a 32 x 32 accumulator
-__device__ __forceinline__ int win_acc_row(int i, int l) { return (i & 3) + 8 * (i >> 2) + 4 * (l >> 5); }
 
 // ---- tiles of 64 rows, copied global -> LDS without passing registers ----------------------------------------------------------------------------------
 // The copy is issued from asm, where the compiler does not see it (it would wait for every copy in flight in front of every LDS read).  A ring of NS slots: at

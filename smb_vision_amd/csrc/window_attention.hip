@@ -391,7 +391,9 @@ int window_attention_check(const WinDesc& d, bool backward, const char* what, bo
   if (d.B < 0 || d.Sq < 0 || d.Sk < 0 || d.Hk <= 0 || d.H <= 0 || d.H % d.Hk) { set_error("%s: bad shape B=%d Sq=%d Sk=%d H=%d Hk=%d (H a multiple of Hk)", what, d.B, d.Sq, d.Sk, d.H, d.Hk); return SMBV_ERR_SHAPE; }
   if (d.D <= 0 || d.D > 128 || (d.D & 7)) { set_error("%s: head width %d (a multiple of 8 up to 128)", what, d.D); return SMBV_ERR_SHAPE; }
   if (d.Sk >= (1 << 29) || d.Sq >= (1 << 29) || (unsigned long long)d.Sq * d.G * d.G >= (1ull << 31)) { set_error("%s: Sq=%d Sk=%d with %d heads to a key head is too long for one call", what, d.Sq, d.Sk, d.G); return SMBV_ERR_SHAPE; }
-  if (((unsigned long long)d.Sq * d.G + 63) / 64 * d.Hk * d.B >= (1ull << 30) || ((unsigned long long)d.Sk + 127) / 128 * d.Hk * d.B >= (1ull << 30) || (unsigned long long)d.B * d.H * d.Sq >= (1ull << 40)) { set_error("%s: too many rows for one call", what); return SMBV_ERR_SHAPE; }
+  // a launch has fewer than 2^24 workgroups of 256: 32 rows or 128 keys of one head each, and one pass of the backward 8 lanes or more a row
+  const unsigned long long most = 1ull << 24, heads = (unsigned long long)d.Hk * d.B;
+  if (((unsigned long long)d.Sq * d.G + 31) / 32 * heads >= most || ((unsigned long long)d.Sk + 127) / 128 * heads >= most || (unsigned long long)d.B * d.H * d.Sq >= 16 * most) { set_error("%s: too many rows for one call", what); return SMBV_ERR_SHAPE; }
   if (!(d.scale > 0.f) || !(d.scale < INFINITY)) { set_error("%s: scale must be positive and finite", what); return SMBV_ERR_ARG; }
   if (d.sinks < 0) { set_error("%s: sinks must not be negative", what); return SMBV_ERR_ARG; }
   if (sizes_only) return SMBV_OK;

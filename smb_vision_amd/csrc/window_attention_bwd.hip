@@ -296,7 +296,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
       unit = emax == WIN_NO_EXP ? 1.f : ldexpf(1.f, -emax);
     }
     // 32 rows at a time: qt's products over the channels, its P and dS, its products over the rows.  The matrix pipe runs beside the vector unit when their
-    // instructions alternate (8 products and 64 others: 173 us together, 125 and 115 alone), so each half's vector work stands next to the other's products.
+    // instructions alternate (8 products and 64 others: 173 ns together, 125 and 115 alone, two waves a SIMD), so each half's vector work stands next to the other's products.
     f32x16 s[2], dp[2];
     u32x4 qa[2][KS], ga[2][KS];
     v8 pf[2][2], ds[2][2];

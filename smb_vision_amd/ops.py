@@ -436,7 +436,7 @@ def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_l
     q [B, Sq, H, D], k / v [B, Sk, Hk, D] (bf16 or fp16, any batch / row / head strides that are multiples of 8 elements, H a multiple of Hk, D a multiple of 8
     up to 128).  Query i stands at position p = i + k_len - q_len and sees key j iff j < k_len, j <= p + right (right < 0: no bound; 0: causal) and
     (j >= p - left (left < 0: no bound) or j < sinks).  q_lens / k_lens: int32 [B] on the device (None: Sq / Sk), so the queries are the last rows of their
-    sequence: all of them in training, the newest tokens against a cache in serving (Sq = 1).  A row that sees nothing, padded rows included, is 0 with lse -inf.
+    sequence: all of them in training, the newest tokens against a cache in serving (Sq = 1; the whole cache with k_lens keeps the call's signature).  A row that sees nothing, padded rows included, is 0 with lse -inf.
     Keys that no row of a call can see do not take part, whatever they hold; a NaN or infinity in a value that SOME rows see can reach other rows near them.
 
     Returns (o [B, Sq, H, D], lse fp32 [B, H, Sq]) and with ``resid`` also the residual of o's rounding, which window_attention_bwd takes as ``o_lo``.
@@ -568,6 +568,8 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
                 in_place = t.data_ptr() == like.data_ptr() and list(_ll3(t)) == list(_ll3(like))
                 # (in place beside the other operand's columns of one packed projection is fine: the elements are apart)
                 _writable(t, f"out of {name}", (pos, inv_freq) if in_place else (q, k, pos, inv_freq))
+        if ko is not None and ko.data_ptr() == qo.data_ptr() and qo.numel() and ko.numel():
+            raise ValueError("out: two tensors")
     a = _lib.RopeAxesCfg.from_buffer_copy(plan.args)
     a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), pos.data_ptr(), inv_freq.data_ptr()
     _call(plan, "smbv_rope_axes", a, q.device, workspace=False)
@@ -636,7 +638,7 @@ def gated_norm_fwd(h, x, *, post="rms", post_w=None, post_b=None, gate=None, res
     def make():
         a, lead, d = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
         if out is not None:
-            if (y is None) != (pre is None):
+            if x1 is None or (y is None) != (pre is None):
                 raise ValueError("out: (x1, y), y None exactly when there is no norm in front of the next block")
             _need_gpu(x1, y)
             _same_device(h, x1, y)
@@ -675,6 +677,8 @@ def gated_norm_bwd(dx1, dy, h, x, stats, *, post="rms", post_w=None, post_b=None
         _same_device(h, dx1, dy, stats, dh, dx)
         if (dy is None) != (pre is None) or (dx1 is None and dy is None):
             raise ValueError("dy: given exactly when there is a norm in front of the next block; without it dx1 is needed")
+        if out is not None and (dh is None or dx is None):
+            raise ValueError("out: (dh, dx)")
         if stats.dtype != torch.float32 or tuple(stats.shape) != (a.rows, 4) or not stats.is_contiguous():
             raise ValueError(f"stats: a contiguous fp32 tensor of shape {(a.rows, 4)}")
         if dx1 is not None:

@@ -43,6 +43,15 @@ def test_window_attention_backward_refusals(bad):
     assert _lib.load().smbv_window_attention_bwd(C.byref(attn(**bad)), P, 1 << 40, None) < 0
 
 
+@pytest.mark.parametrize("many", [dict(B=1 << 23, Hk=2), dict(Sk=1 << 28, B=8), dict(B=1 << 12, H=1024, Hk=1, Sq=64)], ids=str)
+def test_window_attention_more_rows_than_a_launch_takes(many):
+    lib = _lib.load()
+    for fn in ("smbv_window_attention_fwd", "smbv_window_attention_bwd"):
+        assert getattr(lib, fn + "_workspace_bytes")(C.byref(attn(**many))) == 0
+        assert getattr(lib, fn)(C.byref(attn(**many)), P, 1 << 60, None) < 0 and "many" in _lib.last_error()
+    assert lib.smbv_rope_axes(C.byref(rope(B=1 << 10, S=(1 << 21) - 1, Dh=1024, section=sec(512, 0, 0, 0))), None) < 0 and "many" in _lib.last_error()
+
+
 def test_workspaces():
     lib = _lib.load()
     a = attn()
@@ -200,6 +209,20 @@ def test_rope_axes_partial_overlap(dry):
     buf = Z(1, 5, 2, 64)
     with pytest.raises(ValueError):
         ops.rope_axes(buf[:, :4], None, Z(1, 4, dtype=torch.int32), Z(32), (32,), out=(buf[:, 1:], None))
+
+
+def test_outputs_are_tensors_of_their_own(dry):
+    q, k, pos = Z(1, 4, 1, 64), Z(1, 4, 1, 64), Z(1, 4, dtype=torch.int32)
+    same = Z(1, 4, 1, 64)
+    with pytest.raises(ValueError):
+        ops.rope_axes(q, k, pos, Z(32), (32,), out=(same, same))
+    a = dict(GOOD)
+    h, x = a.pop("h"), a.pop("x")
+    with pytest.raises(ValueError):
+        ops.gated_norm_fwd(h, x, out=(None, h.clone()), **a)
+    for out in ((None, x.clone()), (h.clone(), None)):
+        with pytest.raises(ValueError):
+            ops.gated_norm_bwd(x.clone(), h.clone(), h, x, Z(12, 4), out=out, **a)
 
 
 GOOD = dict(h=Z(2, 6, 64, dtype=BF), x=Z(2, 6, 64), post="rms", pre="layer", post_w=Z(64), post_b=None, gate=Z(2, 64), pre_w=Z(64), pre_b=Z(64))
