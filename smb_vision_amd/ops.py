@@ -311,7 +311,7 @@ def colsum_bf16(X):
 
 # ---- operators of a transformer block over long token sequences: windowed attention with sinks, rotary positions with several axes, gated norms ------------
 # A call's checks and its C arguments but for the addresses follow from shapes, strides, types and numbers alone: they are worked out once for each such
-# signature (a call for one token is bound by what the host does for it: 38 -> 12 us).
+# signature (a call for one token is bound by what the host does for it: 38 us without, 9 with, 3.5 of them the launch).
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 _EL16 = {torch.bfloat16: 0, torch.float16: 1}
 _EL = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -322,26 +322,42 @@ def _meta(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
+def _packed(shape):
+    """The strides of a contiguous tensor."""
+    out, n = [], 1
+    for x in reversed(shape):
+        out.append(n)
+        n *= max(x, 1)
+    return tuple(reversed(out))
+
+
 class _Plan:
-    """One signature's C arguments without addresses; the entry point and its workspace's size once it has been called."""
-    __slots__ = ("args", "fn", "ws_bytes")
+    """One signature's C arguments without addresses, and the outputs to allocate; the entry point and its workspace's size once it has been called."""
+    __slots__ = ("args", "new", "fn", "ws_bytes")
 
-    def __init__(self, args):
+    def __init__(self, args, device, *new):
         self.args, self.fn, self.ws_bytes = args, None, 0
+        # (a stated layout is the quickest way to an empty tensor: 1.3 us; torch.empty 1.8)
+        self.new = [(tuple(shape), _packed(shape), dtype, device) for shape, dtype in new]
+
+    def empty(self, i):
+        shape, stride, dtype, device = self.new[i]
+        return _empty_strided(shape, stride, dtype=dtype, device=device)
 
 
-def _planned(key, make):
-    plan = _PLANS.get(key)
-    if plan is None:
-        if len(_PLANS) >= 1024:
-            _PLANS.clear()
-        plan = _PLANS[key] = _Plan(make())
+_empty_strided = torch.empty_strided
+
+
+def _keep(key, plan):
+    if len(_PLANS) >= 1024:
+        _PLANS.clear()
+    _PLANS[key] = plan
     return plan
 
 
 def _call(plan, name, args, device, workspace=True):
     """The entry point on the tensors' device and the current stream."""
-    if torch.cuda.current_device() != device.index:
+    if torch._C._cuda_getDevice() != device.index:
         with torch.cuda.device(device):
             return _call(plan, name, args, device, workspace)
     if plan.fn is None:
@@ -442,27 +458,28 @@ def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_l
     Returns (o [B, Sq, H, D], lse fp32 [B, H, Sq]) and with ``resid`` also the residual of o's rounding, which window_attention_bwd takes as ``o_lo``.
     out: a tensor for o (its strides free; with ``resid`` the residual gets a tensor of the same strides)."""
     left, right, sinks, scale = int(left), int(right), int(sinks), None if scale is None else float(scale)
-
-    def make():
+    device = q.device
+    key = ("window_fwd", q.shape, q.stride(), q.dtype, device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+           left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(out))
+    plan = _PLANS.get(key)
+    if plan is None:
         a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
         if out is not None:
             _need_gpu(out)
             _same_device(q, out)
             _heads4(out, "out", q.shape, q.dtype)
         a.so = _ll3_packed(q.shape) if out is None else _ll3(out)
-        return a
-
-    plan = _planned(("window_fwd", _meta(q), _meta(k), _meta(v), left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(out)), make)
+        plan = _keep(key, _Plan(a, device, (q.shape, q.dtype), ((a.B, a.H, a.Sq), torch.float32)))
     if out is None:
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o = plan.empty(0)
     else:
         _writable(out, "out", (q, k, v))
         o = out
-    o_lo = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device) if resid else None
-    lse = torch.empty((plan.args.B, plan.args.H, plan.args.Sq), dtype=torch.float32, device=q.device)
+    o_lo = _empty_strided(o.shape, o.stride(), dtype=o.dtype, device=device) if resid else None
+    lse = plan.empty(1)
     a = _lib.WindowAttn.from_buffer_copy(plan.args)
     a.q_lens, a.k_lens, a.q, a.k, a.v, a.o, a.o_lo, a.lse = _p(q_lens), _p(k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(o_lo), lse.data_ptr()
-    _call(plan, "smbv_window_attention_fwd", a, q.device)
+    _call(plan, "smbv_window_attention_fwd", a, device)
     return (o, lse, o_lo) if resid else (o, lse)
 
 
@@ -472,8 +489,10 @@ def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, sca
     gradients, for instance the column blocks of one packed gradient."""
     left, right, sinks, scale = int(left), int(right), int(sinks), None if scale is None else float(scale)
     outs = (None,) * 3 if out is None else tuple(out)
-
-    def make():
+    key = ("window_bwd", _meta(q), _meta(k), _meta(v), _meta(o), _meta(do), _meta(lse), left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(o_lo),
+           out is None, *(_meta(t) for t in outs))
+    plan = _PLANS.get(key)
+    if plan is None:
         a = _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens)
         _need_gpu(o, do, lse, o_lo)
         _same_device(q, o, do, lse, o_lo)
@@ -493,13 +512,9 @@ def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, sca
                 _heads4(t, name, like.shape, q.dtype)
         a.so, a.sdo = _ll3(o), _ll3(do)
         a.sdq, a.sdk, a.sdv = (_ll3_packed(like.shape) if t is None else _ll3(t) for t, like in zip(outs, (q, k, v)))
-        return a
-
-    key = ("window_bwd", _meta(q), _meta(k), _meta(v), _meta(o), _meta(do), _meta(lse), left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(o_lo),
-           out is None, *(_meta(t) for t in outs))
-    plan = _planned(key, make)
+        plan = _keep(key, _Plan(a, q.device, *((t.shape, q.dtype) for t in (q, k, v))))
     if out is None:
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = plan.empty(0), plan.empty(1), plan.empty(2)
     else:
         dq, dk, dv = outs
         for name, t in zip(("dq", "dk", "dv"), outs):
@@ -519,10 +534,13 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
     in order; inv_freq: fp32 [sum(sections)].  Pair p turns by pos[its axis] * inv_freq[p]; the first 2 * sum(sections) channels of a head are the pairs
     (p, p + sum(sections)), or (2p, 2p + 1) with ``interleaved``; the rest stays.  transpose: the inverse turn - what a gradient goes through on the way back.
     Returns (q', k'); out: tensors for them, (q, k) themselves to turn in place."""
-    sections = tuple(int(n) for n in sections)
+    sections = tuple(map(int, sections))
     qo, ko = (None, None) if out is None else out
-
-    def make():
+    device = q.device
+    key = ("rope_axes", q.shape, q.stride(), q.dtype, device, _meta(k), pos.shape, pos.stride(), pos.dtype, pos.device, inv_freq.shape, inv_freq.stride(),
+           inv_freq.dtype, inv_freq.device, sections, interleaved, transpose, out is None, _meta(qo), _meta(ko))
+    plan = _PLANS.get(key)
+    if plan is None:
         _need_gpu(q, k, pos, inv_freq)
         _same_device(q, k, pos, inv_freq)
         if q.dtype not in _EL:
@@ -556,12 +574,10 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
                 _same_device(q, t)
                 _heads4(t, f"out of {name}", like.shape, q.dtype)
         a.spos = _lib.c_ll3(pos.stride(0), pos.stride(1) if pos.dim() == 3 else 0, pos.stride(-1))
-        return a
-
-    plan = _planned(("rope_axes", _meta(q), _meta(k), _meta(pos), _meta(inv_freq), sections, bool(interleaved), bool(transpose), out is None, _meta(qo), _meta(ko)), make)
+        plan = _keep(key, _Plan(a, device, (q.shape, q.dtype), *(() if k is None else ((k.shape, q.dtype),))))
     if out is None:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        qo = plan.empty(0)
+        ko = None if k is None else plan.empty(1)
     else:
         for name, t, like in (("q", qo, q), ("k", ko, k)):
             if t is not None:
@@ -572,7 +588,7 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
             raise ValueError("out: two tensors")
     a = _lib.RopeAxesCfg.from_buffer_copy(plan.args)
     a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), pos.data_ptr(), inv_freq.data_ptr()
-    _call(plan, "smbv_rope_axes", a, q.device, workspace=False)
+    _call(plan, "smbv_rope_axes", a, device, False)
     return qo, ko
 
 
@@ -634,8 +650,11 @@ def gated_norm_fwd(h, x, *, post="rms", post_w=None, post_b=None, gate=None, res
     Returns (x1 in x's type, y in h's type or None without ``pre``, stats fp32 [rows, 4] for gated_norm_bwd).  out: (x1, y), x1 may be x itself."""
     eps, res_scale = float(eps), float(res_scale)
     x1, y = (None, None) if out is None else out
-
-    def make():
+    device = h.device
+    key = ("gated_norm_fwd", h.shape, h.stride(), h.dtype, device, x.shape, x.stride(), x.dtype, x.device, post, _meta(post_w), _meta(post_b), _meta(gate), res_scale,
+           pre, _meta(pre_w), _meta(pre_b), eps, out is None, _meta(x1), _meta(y))
+    plan = _PLANS.get(key)
+    if plan is None:
         a, lead, d = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
         if out is not None:
             if x1 is None or (y is None) != (pre is None):
@@ -644,23 +663,20 @@ def gated_norm_fwd(h, x, *, post="rms", post_w=None, post_b=None, gate=None, res
             _same_device(h, x1, y)
         a.ldx1 = d if x1 is None else _rows2(x1, "x1", lead, d, x.dtype)
         a.ldy = d if y is None else _rows2(y, "y", lead, d, h.dtype)
-        return a
-
-    plan = _planned(("gated_norm_fwd", _meta(h), _meta(x), post, _meta(post_w), _meta(post_b), _meta(gate), res_scale, pre, _meta(pre_w), _meta(pre_b), eps,
-                         out is None, _meta(x1), _meta(y)), make)
+        plan = _keep(key, _Plan(a, device, (x.shape, x.dtype), (h.shape, h.dtype), ((a.rows, 4), torch.float32)))
     if out is None:
-        x1 = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        y = torch.empty(h.shape, dtype=h.dtype, device=h.device) if pre else None
+        x1 = plan.empty(0)
+        y = plan.empty(1) if pre else None
     else:
         params = (h, post_w, post_b, gate, pre_w, pre_b)
         _writable(x1, "x1", params if x1.data_ptr() == x.data_ptr() and plan.args.ldx1 == plan.args.ldx else (*params, x))
         if y is not None:
             _writable(y, "y", (*params, x, x1))
-    stats = torch.empty((plan.args.rows, 4), dtype=torch.float32, device=h.device)
+    stats = plan.empty(2)
     a = _lib.GatedNorm.from_buffer_copy(plan.args)
     a.h, a.x, a.post_w, a.post_b, a.gate, a.pre_w, a.pre_b = h.data_ptr(), x.data_ptr(), _p(post_w), _p(post_b), _p(gate), _p(pre_w), _p(pre_b)
     a.x1, a.y, a.stats = x1.data_ptr(), _p(y), stats.data_ptr()
-    _call(plan, "smbv_gated_norm_fwd", a, h.device, workspace=False)
+    _call(plan, "smbv_gated_norm_fwd", a, device, False)
     return x1, y, stats
 
 
@@ -670,8 +686,10 @@ def gated_norm_bwd(dx1, dy, h, x, stats, *, post="rms", post_w=None, post_b=None
     gradient under its name ("gate", "post_w", "post_b", "pre_w", "pre_b"; None for the others).  The same call gives the same bits.  out: (dh, dx)."""
     res_scale = float(res_scale)
     dh, dx = (None, None) if out is None else out
-
-    def make():
+    key = ("gated_norm_bwd", _meta(dx1), _meta(dy), _meta(h), _meta(x), _meta(stats), post, _meta(post_w), _meta(post_b), _meta(gate), res_scale,
+           pre, _meta(pre_w), _meta(pre_b), out is None, _meta(dh), _meta(dx))
+    plan = _PLANS.get(key)
+    if plan is None:
         a, lead, d = _gated_norm_args(h, x, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, 0.0)
         _need_gpu(dx1, dy, stats, dh, dx)
         _same_device(h, dx1, dy, stats, dh, dx)
@@ -687,12 +705,9 @@ def gated_norm_bwd(dx1, dy, h, x, stats, *, post="rms", post_w=None, post_b=None
             a.lddy = _rows2(dy, "dy", lead, d, h.dtype)
         a.lddh = d if out is None else _rows2(dh, "dh", lead, d, h.dtype)
         a.lddx = d if out is None else _rows2(dx, "dx", lead, d, x.dtype)
-        return a
-
-    plan = _planned(("gated_norm_bwd", _meta(dx1), _meta(dy), _meta(h), _meta(x), _meta(stats), post, _meta(post_w), _meta(post_b), _meta(gate), res_scale,
-                                   pre, _meta(pre_w), _meta(pre_b), out is None, _meta(dh), _meta(dx)), make)
+        plan = _keep(key, _Plan(a, h.device, (h.shape, h.dtype), (x.shape, x.dtype)))
     if out is None:
-        dh, dx = torch.empty(h.shape, dtype=h.dtype, device=h.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dh, dx = plan.empty(0), plan.empty(1)
     else:
         ins = (h, x, dx1, dy, stats, post_w, post_b, gate, pre_w, pre_b)
         _writable(dh, "dh", (*ins, dx))
