@@ -103,6 +103,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
     if constexpr (E::half) {
 #pragma unroll
       for (int k = 0; k < 8; k++) gf[ks][k] = (_Float16)ldexpf((float)gf[ks][k], -e);
+      asm volatile("" : "+v"(gf[ks]));
     }
   }
   f32x16 acc[DT], cdel;   // cdel: -delta, the start of every dP product
@@ -152,7 +153,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
   if (nt > 0) win_walk<NS, 2 * IMG>(nt, win_arrived<(NS - 2) * 2 * Copy::NP>, stage, keys, [&](int by) { rd.move(by); });
   if (r >= rows) return;
   uint16_t* out = d.dq + b * d.sdq.b + i * d.sdq.r + head * d.sdq.h;
-  const float f = E::half ? ldexpf(d.scale, e) : d.scale;
+  float f = d.scale;
+  if (E::half && live) {   // (read again: a register less in the walk)
+    e = wrows.expo[((long long)b * d.Hk + hk) * rows + r];
+    if (e != WIN_NO_EXP) f = ldexpf(f, e);
+  }
 #pragma unroll
   for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -283,9 +288,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     float unit = 1.f;
     if constexpr (E::half) {
       int e = *(const int*)(st + 512 + 4 * l);
+      if (__builtin_amdgcn_ballot_w64(e > emax) != 0) {   // (seldom after the first tiles)
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 64));
-      if (e > emax) {
+        for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 64));
         const float f = emax == WIN_NO_EXP ? 0.f : ldexpf(1.f, emax - e);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
