@@ -140,9 +140,9 @@ template <int DP> struct WinRead {
   // (an LDS instruction's immediate reaches 64 KiB: a ring of 128 KiB is read from one half, then the other)
   __device__ __forceinline__ void move(int by) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) row[ks] += by;
+    for (int ks = 0; ks < KS; ks++) { row[ks] += by; asm volatile("" : "+v"(row[ks])); }   // (or it is added at every read)
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) { tr[dt][0] += by; tr[dt][1] += by; }
+    for (int dt = 0; dt < DT; dt++) { tr[dt][0] += by; tr[dt][1] += by; asm volatile("" : "+v"(tr[dt][0]), "+v"(tr[dt][1])); }
   }
 };
 __device__ __forceinline__ void win_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }  // (no copy may outlive its workgroup)

@@ -191,7 +191,7 @@ struct WinSplit {
 __device__ __host__ __forceinline__ int win_split_slots(const WinSplit& s) { return (s.c1 > 1 ? s.nsink * s.c1 : 0) + (s.c2 > 1 ? (s.tiles - s.nsink) * s.c2 : 0); }
 
 // Heads wider than 64 keep 192 registers of accumulators and of K and V: one wave a SIMD with all the registers, reading its operands ahead of their products,
-// beats both two waves that spill (1164 us against 696 at 4 x 4093 tokens, 16 heads on 4 of 128) and workgroups of their own for dK and dV, which form S twice.
+// beats both two waves that spill (1164 us against 696 for a pass at 4 x 4093 tokens, 16 heads on 4 of 128) and workgroups of their own for dK and dV, which form S twice.
 template <class E, int DP, int NW, int NS>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 ? 1 : 2, DP == 128 ? 1 : 2))) void win_dkv_kernel(WinDesc d, WinRows wrows, WinSplit sp) {
   constexpr int KS = DP / 16, DT = DP / 32, IMG = 64 * DP * 2, BK = 32 * NW, SLOT = 2 * IMG, STAT = NS * SLOT;   // STAT: where the rows' numbers lie
@@ -363,7 +363,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
           dk[dt] = E::mfma(__builtin_bit_cast(v8, qc[qt][half][dt]), ds[qt][half], dk[dt]);
         }
     };
-    constexpr int VALU = E::half ? 72 : 56;   // of probs
+    // Vector instructions behind a product: as many as probs has between them - but at one wave a SIMD, where both compete for issue, two beside the scores
+    // (whose products the probabilities wait for) and six beside the gradients (4 x 4093 tokens, 16 heads on 4 of 128: 3 and 3 322 us, 4 and 4 313, 2 and 6 299)
+    constexpr int VALU = E::half ? 72 : 56;
     rows(0);
     if constexpr (AHEAD) WIN_AHEAD();
     rows(1);
@@ -372,12 +374,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     cols(0);
     scores(1);
     probs(0);
-    win_weave<2 * KS, VALU / (2 * KS)>();
+    win_weave<2 * KS, DP == 128 ? 2 : VALU / (2 * KS)>();
     if (!all) mask(1);
     cols(1);
     grads(0);
     probs(1);
-    win_weave<4 * DT, VALU / (4 * DT)>();
+    win_weave<4 * DT, DP == 128 ? 6 : VALU / (4 * DT)>();
     grads(1);
   };
   if (rlo < rhi) win_walk<NS, SLOT>((rhi - rlo + 63) / 64, win_arrived<(NS - 2) * (2 * Copy::NP + 1)>, stage, rowtile, [&](int by) { rd.move(by); });
