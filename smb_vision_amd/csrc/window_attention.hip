@@ -415,7 +415,9 @@ int window_attention_check(const WinDesc& d, bool backward, const char* what, bo
 }
 
 // Up to 64 rows a key head go to the 32-row kernel: at 128 rows most of a workgroup would have none.  Shares: as many as bring every CU the workgroups that it
-// holds (by LDS and registers: one at 128 channels and few rows, else two or three), none with less than 256 (512) keys, which cost about what a share's sums do.
+// holds (by LDS and registers: one at 128 channels and few rows, else two or three), none with less than 256 (512) keys, which cost about what a share's sums do
+// (two caches of 4001 keys, 16 heads on 4 of 80, window 1500, in a replayed graph: 12 queries, at least 128 keys a share 15.1 us, 256 14.8, 512 17.1;
+// 333 queries, at least 256 keys 37.8 us, 512 33.7, 1024 41.6).
 struct WinPlan { bool few; int shares; };
 static WinPlan win_plan(const WinDesc& d) {
   const long long rows = (long long)d.Sq * d.G, heads = (long long)d.Hk * d.B;
