@@ -421,6 +421,24 @@ def _writable(t, name, inputs=()):
                 raise ValueError(f"{name}: an output must not overlap an operand")
 
 
+def _apart(*ts):
+    """Outputs [B, S, H, D] of one call lie apart: nowhere near each other, or as columns of one packed tensor (equal steps between rows, other places in them)."""
+    ts = [t for t in ts if t is not None and t.numel()]
+    for n, a in enumerate(ts):
+        for b in ts[n + 1:]:
+            (lo, hi), (lo2, hi2) = _extent(a), _extent(b)
+            if hi <= lo2 or hi2 <= lo:
+                continue
+            steps = [i for i in (0, 1) if a.shape[i] > 1 or b.shape[i] > 1]
+            row = min((a.stride(i) for i in steps), default=0)
+            wa, wb = ((t.shape[2] - 1) * t.stride(2) + t.shape[3] for t in (a, b))
+            if row > 0 and all(a.stride(i) == b.stride(i) and a.stride(i) % row == 0 for i in steps):
+                at = (lo2 - lo) // a.element_size() % row
+                if at >= wa and at + wb <= row:
+                    continue
+            raise ValueError("out: tensors that share no memory")
+
+
 def _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens):
     _need_gpu(q, k, v, q_lens, k_lens)
     _same_device(q, k, v, q_lens, k_lens)
@@ -519,8 +537,7 @@ def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, sca
         dq, dk, dv = outs
         for name, t in zip(("dq", "dk", "dv"), outs):
             _writable(t, name, (q, k, v, o, do, o_lo, lse))
-        if len({t.data_ptr() for t in outs if t.numel()}) < sum(t.numel() > 0 for t in outs):
-            raise ValueError("out: three tensors")
+        _apart(*outs)
     a = _lib.WindowAttn.from_buffer_copy(plan.args)
     a.q_lens, a.k_lens, a.q, a.k, a.v = _p(q_lens), _p(k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.o, a.o_lo, a.lse, a.d_o, a.dq, a.dk, a.dv = o.data_ptr(), _p(o_lo), lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
@@ -584,8 +601,7 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
                 in_place = t.data_ptr() == like.data_ptr() and list(_ll3(t)) == list(_ll3(like))
                 # (in place beside the other operand's columns of one packed projection is fine: the elements are apart)
                 _writable(t, f"out of {name}", (pos, inv_freq) if in_place else (q, k, pos, inv_freq))
-        if ko is not None and ko.data_ptr() == qo.data_ptr() and qo.numel() and ko.numel():
-            raise ValueError("out: two tensors")
+        _apart(qo, ko)
     a = _lib.RopeAxesCfg.from_buffer_copy(plan.args)
     a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), pos.data_ptr(), inv_freq.data_ptr()
     _call(plan, "smbv_rope_axes", a, device, False)

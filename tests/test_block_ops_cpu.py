@@ -211,11 +211,26 @@ def test_rope_axes_partial_overlap(dry):
         ops.rope_axes(buf[:, :4], None, Z(1, 4, dtype=torch.int32), Z(32), (32,), out=(buf[:, 1:], None))
 
 
-def test_outputs_are_tensors_of_their_own(dry):
+def test_outputs_are_tensors_of_their_own(dry, monkeypatch):
+    made = []
+    monkeypatch.setattr(ops, "_call", lambda plan, name, *a, **kw: made.append(name))
     q, k, pos = Z(1, 4, 1, 64), Z(1, 4, 1, 64), Z(1, 4, dtype=torch.int32)
     same = Z(1, 4, 1, 64)
     with pytest.raises(ValueError):
         ops.rope_axes(q, k, pos, Z(32), (32,), out=(same, same))
+    packed = Z(2, 4, 6, 64)
+    pos = Z(1, 2, 4, dtype=torch.int32)
+    for a, b in ((packed[:, :, :4], packed[:, :, 3:5]), (packed[:, :, 2:], packed[:, :, :3]), (packed[:, :3], packed[:, 1:]), (packed, packed)):
+        with pytest.raises(ValueError):   # turned in place, some heads twice
+            ops.rope_axes(a, b, pos[..., :a.shape[1]], Z(32), (32,), out=(a, b))
+    ops.rope_axes(packed[:, :, :4], packed[:, :, 4:], pos, Z(32), (32,), out=(packed[:, :, :4], packed[:, :, 4:]))   # the columns of one packed tensor
+    q, k, v = (Z(2, 4, n, 64, dtype=BF) for n in (2, 1, 1))
+    o, lse, grad = q.clone(), Z(2, 2, 4), Z(2, 4, 4, 64, dtype=BF)
+    ops.window_attention_bwd(q, k, v, o, o.clone(), lse, out=(grad[:, :, :2], grad[:, :, 2:3], grad[:, :, 3:]))
+    assert made == ["smbv_rope_axes", "smbv_window_attention_bwd"]
+    for a, b, c in ((2, 2, 3), (1, 4, 3)):   # dk inside dq, dk on dv
+        with pytest.raises(ValueError):
+            ops.window_attention_bwd(q, k, v, o, o.clone(), lse, out=(grad[:, :, a - 1:a + 1], grad[:, :, b - 1:b], grad[:, :, c:]))
     a = dict(GOOD)
     h, x = a.pop("h"), a.pop("x")
     with pytest.raises(ValueError):
