@@ -16,7 +16,9 @@ No fallback: anything the kernels do not compute (masks, dropout, causal, head w
 
 `register_window()` adds "smbv_window": smbv_window_attention_fwd / _bwd under the same interface - a sliding window (bound at registration, or the model's own
 `sliding_window`), first tokens that stay visible, causal models, grouped key heads, queries at the end of a longer cache, bf16 and fp16, head widths that are
-multiples of 8 up to 128 - and without copies, since those kernels take the head-major strides as they are.
+multiples of 8 up to 128 - and without copies, since those kernels take the head-major strides as they are.  With the name goes a mask function: a model that
+builds masks has them turned into the window that they say, and one that is no window of full sequences (padding, packed documents, blocks, a cache with empty
+slots) raises.
 """
 import functools
 
@@ -105,6 +107,73 @@ class _SmbvWindowAttentionFn(torch.autograd.Function):
         return (*ops.window_attention_bwd(q, k, v, out, _rows_of_heads(d_out.to(q.dtype)), lse, o_lo=out_lo, **ctx.kw), None)
 
 
+def _on_gpu(t):
+    return t.is_cuda
+
+
+class _WindowMask:
+    """What a model's mask says: query i, at position p = i + keys - queries, sees key j iff p - left <= j <= p + right (-1: no bound)."""
+    __slots__ = ("queries", "keys", "left", "right")
+
+    def __init__(self, queries, keys, left, right):
+        self.queries, self.keys, self.left, self.right = queries, keys, left, right
+
+
+_EMPTY_SLOTS = "smbv window attention: {} positions hold tokens and there are {} keys: no preallocated cache with empty slots"
+
+
+def _window_mask(*, batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function, attention_mask=None, device=None, **unused):
+    """transformers mask-interface function: the window that `mask_function(batch, head, query, key)` is over these queries and keys, as a _WindowMask.
+
+    The last query's first key and the first query's last key give the two bounds (none where they reach the ends); every query then has to see the first and the
+    last key of its window and nothing next to it, which a padded, packed or blocked mask does not pass.  attention_mask: which positions hold tokens - all."""
+    n, m, q0, k0 = int(q_length), int(kv_length), int(q_offset), int(kv_offset)
+    if attention_mask is not None:
+        if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("smbv window attention: a padding mask cannot be looked at inside a graph capture; pass none (every position holds a token)")
+        if attention_mask.shape[-1] < k0 + m:
+            raise ValueError(_EMPTY_SLOTS.format(attention_mask.shape[-1], k0 + m))
+        if attention_mask.dim() != 2 or not bool(attention_mask[:, k0:k0 + m].all()):
+            raise ValueError("smbv window attention: padded batches are not supported (every position of the attention mask has to hold a token); "
+                             "ops.window_attention_fwd takes per-sequence lengths")
+
+    def sees(dev, qi, kj):
+        b = torch.arange(int(batch_size), device=dev).view(-1, 1, 1)
+        qi, kj = qi.to(dev), kj.to(dev)
+        r = mask_function(b, torch.zeros((), dtype=torch.long, device=dev), qi + q0, kj + k0)
+        return r.broadcast_to(torch.broadcast_shapes(r.shape, b.shape, qi.shape, kj.shape)).cpu()
+
+    def window(dev):
+        if n == 0 or m == 0:
+            return -1, -1
+        i, j = torch.arange(n).view(1, n, 1), torch.arange(m).view(1, 1, m)
+        first, last = sees(dev, i[:, :1], j)[0, 0].nonzero(), sees(dev, i[:, -1:], j)[0, 0].nonzero()
+        if first.numel() == 0 or last.numel() == 0:
+            return None
+        lo, hi = int(last[0]), int(first[-1])
+        left, right = -1 if lo == 0 else m - 1 - lo, -1 if hi == m - 1 else hi - (m - n)
+        if (lo and left < 0) or (hi < m - 1 and right < 0) or last.numel() != int(last[-1]) - lo + 1 or first.numel() != hi - int(first[0]) + 1:
+            return None
+        p = i + (m - n)
+        a = torch.zeros_like(p) if left < 0 else (p - left).clamp(min=0)
+        z = torch.full_like(p, m - 1) if right < 0 else (p + right).clamp(max=m - 1)
+        inside = sees(dev, i, torch.cat([a, (a + z) // 2, z], 2)).all()
+        outside = (sees(dev, i, (a - 1).clamp(min=0)) & (a > 0)).any() | (sees(dev, i, (z + 1).clamp(max=m - 1)) & (z < m - 1)).any()
+        return (left, right) if bool(inside) and not bool(outside) else None
+
+    try:   # (in host memory, without waiting for the device - unless the function looks something up there)
+        found = window("cpu")
+    except RuntimeError:
+        if device is None or torch.device(device).type == "cpu":
+            raise
+        found = window(device)
+    if found != (-1, -1) and q0 - k0 != m - n:
+        raise ValueError(_EMPTY_SLOTS.format(q0 - k0 + n, m))
+    if found is None:
+        raise ValueError("smbv window attention: the model's mask is no sliding window over full sequences (packed documents, blocks and prefixes are not supported)")
+    return _WindowMask(n, m, *found)
+
+
 def _rows_of_heads(t):
     """t [B, S, H, D] as the kernels can read it: contiguous channels, 16-byte steps."""
     if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3)):
@@ -117,8 +186,30 @@ def smbv_window_attention(module, query, key, value, attention_mask=None, *, sca
 
     sliding_window: None, or W - keys closer than W positions, in both directions unless the attention is causal -, or (left, right) - as many keys to either
     side, -1 for all.  is_causal: None takes the module's own `is_causal` (False if it has none).  The queries are the last Sq of the Sk positions, all of which
-    hold tokens: no preallocated cache with empty slots.  sinks: first keys that stay visible to every later query.  fp32 operands are rounded to bf16."""
-    if attention_mask is not None:
+    hold tokens: no preallocated cache with empty slots.  sinks: first keys that stay visible to every later query.  fp32 operands are rounded to bf16.
+    attention_mask: None, or what the mask function of register_window() made of the model's mask, which then says what is seen in place of is_causal and of the
+    model's own sliding_window."""
+    return _window_attention(module, query, key, value, attention_mask, scaling, dropout, is_causal, sliding_window, None, sinks)
+
+
+def _bounds(window):
+    if window is None:
+        return -1, -1
+    if isinstance(window, int):
+        if window < 1:
+            raise ValueError(f"smbv window attention: sliding_window {window}")
+        return window - 1, window - 1
+    left, right = (int(x) for x in window)
+    return left, right
+
+
+def _narrower(a, b):
+    return max(a, b) if a < 0 or b < 0 else min(a, b)
+
+
+def _window_attention(module, query, key, value, mask, scaling, dropout, is_causal, sliding_window, bound, sinks):
+    """bound: the window of register_window(), for models that pass no `sliding_window`."""
+    if mask is not None and not isinstance(mask, _WindowMask):
         raise ValueError("smbv window attention: masks are not supported (the window, causality and the first tokens are arguments)")
     if dropout:
         raise ValueError("smbv window attention: attention dropout is not supported")
@@ -127,19 +218,19 @@ def smbv_window_attention(module, query, key, value, attention_mask=None, *, sca
                          f"{tuple(key.shape)}, {tuple(value.shape)}")
     if query.shape[3] % 8 or not 0 < query.shape[3] <= 128:
         raise ValueError(f"smbv window attention: head width {query.shape[3]} (a multiple of 8 up to 128)")
-    if not query.is_cuda:
+    if not _on_gpu(query):
         raise RuntimeError("smbv window attention needs an MI355X: there is no CPU path")
-    causal = bool(getattr(module, "is_causal", False) if is_causal is None else is_causal)
-    if sliding_window is None:
-        left = right = -1
-    elif isinstance(sliding_window, int):
-        if sliding_window < 1:
-            raise ValueError(f"smbv window attention: sliding_window {sliding_window}")
-        left = right = sliding_window - 1
+    left, right = _bounds(bound if sliding_window is None else sliding_window)
+    if mask is None:
+        if bool(getattr(module, "is_causal", False) if is_causal is None else is_causal):
+            right = 0
     else:
-        left, right = (int(x) for x in sliding_window)
-    if causal:
-        right = 0
+        if (mask.queries, mask.keys) != (query.shape[2], key.shape[2]):
+            raise ValueError(f"smbv window attention: a mask for {mask.queries} queries and {mask.keys} keys, got {query.shape[2]} and {key.shape[2]}")
+        if sliding_window is not None or bound is None:
+            left, right = mask.left, mask.right
+        else:
+            left, right = _narrower(left, mask.left), _narrower(right, mask.right)
     dtype = query.dtype if query.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
     q, k, v = (_rows_of_heads(t.transpose(1, 2).to(dtype)) for t in (query, key, value))
     kw = dict(left=left, right=right, sinks=int(sinks), scale=None if scaling is None else float(scaling))
@@ -153,11 +244,12 @@ def smbv_window_attention(module, query, key, value, attention_mask=None, *, sca
 def register_window(name=WINDOW_NAME, *, window=None, sinks=0):
     """Make `config._attn_implementation = name` select the windowed kernels.  window: what takes the place of `sliding_window` in models that pass none (the
     reference's encoders among them); sinks: first tokens that stay visible."""
-    from transformers import AttentionInterface
+    from transformers import AttentionInterface, AttentionMaskInterface
 
     @functools.wraps(smbv_window_attention)
-    def attend(module, query, key, value, attention_mask=None, *, sliding_window=None, **kwargs):
-        return smbv_window_attention(module, query, key, value, attention_mask, sliding_window=window if sliding_window is None else sliding_window, sinks=sinks, **kwargs)
+    def attend(module, query, key, value, attention_mask=None, *, scaling=None, dropout=0.0, is_causal=None, sliding_window=None, **kwargs):
+        return _window_attention(module, query, key, value, attention_mask, scaling, dropout, is_causal, sliding_window, window, sinks)
 
     AttentionInterface.register(name, attend)
+    AttentionMaskInterface.register(name, _window_mask)
     return name
