@@ -107,6 +107,17 @@ class _SmbvWindowAttentionFn(torch.autograd.Function):
         return (*ops.window_attention_bwd(q, k, v, out, _rows_of_heads(d_out.to(q.dtype)), lse, o_lo=out_lo, **ctx.kw), None)
 
 
+# Arguments that models hand on and that change nothing here: what positions, masks and outputs they name is settled before the attention or behind it.
+_HARMLESS = {"position_ids", "cache_position", "use_cache", "output_attentions", "output_hidden_states", "output_router_logits", "return_dict",
+             "encoder_hidden_states", "num_items_in_batch"}
+
+
+def _refuse(kwargs):
+    for name, x in kwargs.items():
+        if x is not None and name not in _HARMLESS:
+            raise ValueError(f"smbv window attention: the argument {name!r} is not supported (a cap on the scores, learned sinks, a bias: they change the result)")
+
+
 def _on_gpu(t):
     return t.is_cuda
 
@@ -188,7 +199,8 @@ def smbv_window_attention(module, query, key, value, attention_mask=None, *, sca
     side, -1 for all.  is_causal: None takes the module's own `is_causal` (False if it has none).  The queries are the last Sq of the Sk positions, all of which
     hold tokens: no preallocated cache with empty slots.  sinks: first keys that stay visible to every later query.  fp32 operands are rounded to bf16.
     attention_mask: None, or what the mask function of register_window() made of the model's mask, which then says what is seen in place of is_causal and of the
-    model's own sliding_window."""
+    model's own sliding_window.  Other arguments raise, but for None and a few that change nothing."""
+    _refuse(kwargs)
     return _window_attention(module, query, key, value, attention_mask, scaling, dropout, is_causal, sliding_window, None, sinks)
 
 
@@ -248,6 +260,7 @@ def register_window(name=WINDOW_NAME, *, window=None, sinks=0):
 
     @functools.wraps(smbv_window_attention)
     def attend(module, query, key, value, attention_mask=None, *, scaling=None, dropout=0.0, is_causal=None, sliding_window=None, **kwargs):
+        _refuse(kwargs)
         return _window_attention(module, query, key, value, attention_mask, scaling, dropout, is_causal, sliding_window, window, sinks)
 
     AttentionInterface.register(name, attend)

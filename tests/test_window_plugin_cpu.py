@@ -152,3 +152,23 @@ def test_bound_window_narrows_a_mask(calls, bound, want):
     calls.clear()
     out(ours, IDS)
     assert {c[2:4] for c in calls} == {(7, 0)}
+
+
+@pytest.mark.parametrize("kind,argument", [("gemma2", "softcap"), ("gpt_oss", "s_aux")])
+def test_models_with_another_softmax_are_refused(calls, kind, argument):
+    _, ours = both(kind)
+    with pytest.raises(ValueError, match=argument):
+        out(ours, IDS)
+    assert not calls
+
+
+@pytest.mark.parametrize("extra", [dict(softcap=50.0), dict(s_aux=torch.zeros(2)), dict(position_bias=torch.zeros(1)), dict(head_mask=torch.ones(2)),
+                                   dict(cu_seq_lens_q=torch.tensor([0, 4])), dict(never_heard_of=0)], ids=lambda d: next(iter(d)))
+def test_unknown_arguments_are_refused(calls, extra):
+    q, m = torch.zeros(1, 2, 8, 64), torch.nn.Module()
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+    named = ALL_ATTENTION_FUNCTIONS[attention_plugin.register_window("smbv_window_for_test")]
+    for f in (attention_plugin.smbv_window_attention, named):
+        with pytest.raises(ValueError, match=next(iter(extra))):
+            f(m, q, q, q, **extra)
+        f(m, q, q, q, **{n: None for n in extra}, position_ids=torch.arange(8)[None], use_cache=True)
