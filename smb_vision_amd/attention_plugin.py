@@ -109,7 +109,7 @@ class _SmbvWindowAttentionFn(torch.autograd.Function):
 
 # Arguments that models hand on and that change nothing here: what positions, masks and outputs they name is settled before the attention or behind it.
 _HARMLESS = {"position_ids", "cache_position", "use_cache", "output_attentions", "output_hidden_states", "output_router_logits", "return_dict",
-             "encoder_hidden_states", "num_items_in_batch"}
+             "encoder_hidden_states", "num_items_in_batch", "deterministic"}   # (the kernels always are)
 
 
 def _refuse(kwargs):
