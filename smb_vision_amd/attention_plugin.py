@@ -123,11 +123,12 @@ def _on_gpu(t):
 
 
 class _WindowMask:
-    """What a model's mask says: query i, at position p = i + keys - queries, sees key j iff p - left <= j <= p + right (-1: no bound)."""
-    __slots__ = ("queries", "keys", "left", "right")
+    """What a model's mask says: query i, at position p = i + keys - queries, sees key j iff p - left <= j <= p + right (-1: no bound); `dropped`
+    positions in front of the first key are no longer in the cache."""
+    __slots__ = ("queries", "keys", "left", "right", "dropped")
 
-    def __init__(self, queries, keys, left, right):
-        self.queries, self.keys, self.left, self.right = queries, keys, left, right
+    def __init__(self, queries, keys, left, right, dropped):
+        self.queries, self.keys, self.left, self.right, self.dropped = queries, keys, left, right, dropped
 
 
 _EMPTY_SLOTS = "smbv window attention: {} positions hold tokens and there are {} keys: no preallocated cache with empty slots"
@@ -182,7 +183,7 @@ def _window_mask(*, batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
         raise ValueError(_EMPTY_SLOTS.format(q0 - k0 + n, m))
     if found is None:
         raise ValueError("smbv window attention: the model's mask is no sliding window over full sequences (packed documents, blocks and prefixes are not supported)")
-    return _WindowMask(n, m, *found)
+    return _WindowMask(n, m, *found, k0)
 
 
 def _rows_of_heads(t):
@@ -197,7 +198,9 @@ def smbv_window_attention(module, query, key, value, attention_mask=None, *, sca
 
     sliding_window: None, or W - keys closer than W positions, in both directions unless the attention is causal -, or (left, right) - as many keys to either
     side, -1 for all.  is_causal: None takes the module's own `is_causal` (False if it has none).  The queries are the last Sq of the Sk positions, all of which
-    hold tokens: no preallocated cache with empty slots.  sinks: first keys that stay visible to every later query.  fp32 operands are rounded to bf16.
+    hold tokens: no preallocated cache with empty slots.  sinks: first keys that stay visible to every later query; the cache has to keep them, so a model's own
+    sliding_window, whose cache forgets them, takes sinks only while they are there, and, without a mask to tell, only with as many keys as queries.  fp32
+    operands are rounded to bf16.
     attention_mask: None, or what the mask function of register_window() made of the model's mask, which then says what is seen in place of is_causal and of the
     model's own sliding_window.  Other arguments raise, but for None and a few that change nothing."""
     _refuse(kwargs)
@@ -233,6 +236,8 @@ def _window_attention(module, query, key, value, mask, scaling, dropout, is_caus
     if not _on_gpu(query):
         raise RuntimeError("smbv window attention needs an MI355X: there is no CPU path")
     left, right = _bounds(bound if sliding_window is None else sliding_window)
+    if sinks > 0 and (mask.dropped > 0 if mask is not None else isinstance(sliding_window, int) and key.shape[2] > query.shape[2]):
+        raise ValueError("smbv window attention: sinks with a cache that does not keep the first tokens (use a full cache, the window bound by register_window())")
     if mask is None:
         if bool(getattr(module, "is_causal", False) if is_causal is None else is_causal):
             right = 0
@@ -255,7 +260,8 @@ def _window_attention(module, query, key, value, mask, scaling, dropout, is_caus
 
 def register_window(name=WINDOW_NAME, *, window=None, sinks=0):
     """Make `config._attn_implementation = name` select the windowed kernels.  window: what takes the place of `sliding_window` in models that pass none (the
-    reference's encoders among them); sinks: first tokens that stay visible."""
+    reference's encoders among them); sinks: first tokens that stay visible, with a cache that keeps them (the sliding cache of a model with a window of its own
+    does not: generation past it raises)."""
     from transformers import AttentionInterface, AttentionMaskInterface
 
     @functools.wraps(smbv_window_attention)

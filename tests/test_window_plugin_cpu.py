@@ -172,3 +172,28 @@ def test_unknown_arguments_are_refused(calls, extra):
         with pytest.raises(ValueError, match=next(iter(extra))):
             f(m, q, q, q, **extra)
         f(m, q, q, q, **{n: None for n in extra}, position_ids=torch.arange(8)[None], use_cache=True)
+
+
+def test_sinks_need_a_cache_that_keeps_them(calls):
+    """A full cache with the window bound at registration gives token by token what a prompt gives; a sliding cache, which forgets the first tokens, raises."""
+    _, full = both("llama", window=(7, -1), sinks=4)
+    want, cache, got = out(full, IDS), None, []
+    for n, at in ((12, 0), *((1, i) for i in range(12, 20))):
+        with torch.no_grad():
+            o = full(IDS[:, at:at + n], past_key_values=cache, use_cache=True)
+        cache = o.past_key_values
+        got.append(o.logits)
+    assert rms_err(torch.cat(got, 1), want) < 2e-2 and {c[4] for c in calls} == {4}
+    _, sliding = both("mistral", sinks=4)   # (its window is 8: the cache keeps 7)
+    with torch.no_grad():
+        short = sliding(IDS[:, :6], use_cache=True).past_key_values
+        sliding(IDS[:, 6:7], past_key_values=short, use_cache=True)   # the first tokens are still there
+        long = sliding(IDS[:, :12], use_cache=True).past_key_values
+        with pytest.raises(ValueError, match="first tokens"):
+            sliding(IDS[:, 12:13], past_key_values=long, use_cache=True)
+    q, k, m = torch.zeros(1, 2, 1, 64), torch.zeros(1, 2, 8, 64), torch.nn.Module()
+    with pytest.raises(ValueError, match="first tokens"):
+        attention_plugin.smbv_window_attention(m, q, k, k, sliding_window=8, sinks=4)
+    attention_plugin.smbv_window_attention(m, q, k, k, sliding_window=(7, 0), sinks=4)
+    attention_plugin.smbv_window_attention(m, k, k, k, sliding_window=8, sinks=4)
+    attention_plugin.smbv_window_attention(m, q, k, k, sliding_window=8)
