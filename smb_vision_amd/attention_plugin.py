@@ -92,7 +92,9 @@ def _not_captured():
 
 class _SmbvWindowAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, kw):
+    def forward(ctx, q, k, v, kw, train):
+        if not train:
+            return ops.window_attention_fwd(q, k, v, **kw)[0]
         _not_captured()
         out, lse, out_lo = ops.window_attention_fwd(q, k, v, resid=True, **kw)
         ctx.save_for_backward(q, k, v, out, lse, out_lo)
@@ -104,7 +106,7 @@ class _SmbvWindowAttentionFn(torch.autograd.Function):
     def backward(ctx, d_out):
         _not_captured()
         q, k, v, out, lse, out_lo = ctx.saved_tensors
-        return (*ops.window_attention_bwd(q, k, v, out, _rows_of_heads(d_out.to(q.dtype)), lse, o_lo=out_lo, **ctx.kw), None)
+        return (*ops.window_attention_bwd(q, k, v, out, _rows_of_heads(d_out.to(q.dtype)), lse, o_lo=out_lo, **ctx.kw), None, None)
 
 
 # Arguments that models hand on and that change nothing here: what positions, masks and outputs they name is settled before the attention or behind it.
@@ -251,11 +253,9 @@ def _window_attention(module, query, key, value, mask, scaling, dropout, is_caus
     dtype = query.dtype if query.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
     q, k, v = (_rows_of_heads(t.transpose(1, 2).to(dtype)) for t in (query, key, value))
     kw = dict(left=left, right=right, sinks=int(sinks), scale=None if scaling is None else float(scaling))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out = _SmbvWindowAttentionFn.apply(q, k, v, kw)
-    else:
-        out = ops.window_attention_fwd(q, k, v, **kw)[0]
-    return out.to(query.dtype), None
+    # (through the autograd function also without gradients: forward-mode tangents, which it has no rule for, then raise instead of being dropped)
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return _SmbvWindowAttentionFn.apply(q, k, v, kw, train).to(query.dtype), None
 
 
 def register_window(name=WINDOW_NAME, *, window=None, sinks=0):

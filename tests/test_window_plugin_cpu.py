@@ -197,3 +197,19 @@ def test_sinks_need_a_cache_that_keeps_them(calls):
     attention_plugin.smbv_window_attention(m, q, k, k, sliding_window=(7, 0), sinks=4)
     attention_plugin.smbv_window_attention(m, k, k, k, sliding_window=8, sinks=4)
     attention_plugin.smbv_window_attention(m, q, k, k, sliding_window=8)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_tangents_are_not_dropped(calls, grad):
+    import torch.autograd.forward_ad as fwd
+    x, m = torch.randn(1, 2, 8, 64), torch.nn.Module()
+    for n in range(3):
+        with fwd.dual_level(), torch.set_grad_enabled(grad):
+            t = [x, x, x]
+            t[n] = fwd.make_dual(x, torch.randn_like(x))
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
+                attention_plugin.smbv_window_attention(m, *t)
+    o = attention_plugin.smbv_window_attention(m, x, x, x)[0]
+    assert not o.requires_grad and o.grad_fn is None
+    with torch.no_grad():
+        assert torch.equal(attention_plugin.smbv_window_attention(m, x.clone().requires_grad_(True), x, x)[0], o)
