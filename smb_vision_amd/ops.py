@@ -422,7 +422,8 @@ def _writable(t, name, inputs=()):
 
 
 def _apart(*ts):
-    """Outputs [B, S, H, D] of one call lie apart: nowhere near each other, or as columns of one packed tensor (equal steps between rows, other places in them)."""
+    """Tensors [B, S, H, D] of one call, of which at least one of any two is written, lie apart: nowhere near each other, or as columns of one packed tensor (equal
+    steps between rows, other places in them)."""
     ts = [t for t in ts if t is not None and t.numel()]
     for n, a in enumerate(ts):
         for b in ts[n + 1:]:
@@ -596,11 +597,12 @@ def rope_axes(q, k, pos, inv_freq, sections, *, interleaved=False, transpose=Fal
         qo = plan.empty(0)
         ko = None if k is None else plan.empty(1)
     else:
-        for name, t, like in (("q", qo, q), ("k", ko, k)):
+        for name, t, like, other in (("q", qo, q, k), ("k", ko, k, q)):
             if t is not None:
                 in_place = t.data_ptr() == like.data_ptr() and list(_ll3(t)) == list(_ll3(like))
-                # (in place beside the other operand's columns of one packed projection is fine: the elements are apart)
                 _writable(t, f"out of {name}", (pos, inv_freq) if in_place else (q, k, pos, inv_freq))
+                if in_place:   # beside the other operand's columns of one packed projection is fine, on elements that are still to be read is not
+                    _apart(t, other)
         _apart(qo, ko)
     a = _lib.RopeAxesCfg.from_buffer_copy(plan.args)
     a.q, a.k, a.qo, a.ko, a.pos, a.inv_freq = q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), pos.data_ptr(), inv_freq.data_ptr()

@@ -281,3 +281,19 @@ def test_window_plugin_registers_and_refuses_cpu():
         ALL_ATTENTION_FUNCTIONS[name](torch.nn.Module(), q, q, q, None, scaling=0.125, dropout=0.0)
     with pytest.raises(ValueError):
         ALL_ATTENTION_FUNCTIONS[name](torch.nn.Module(), q, q, q, Z(1, 1, 16, 16))
+
+
+def test_turned_in_place_beside_an_operand_that_is_still_read(dry, monkeypatch):
+    made = []
+    monkeypatch.setattr(ops, "_call", lambda plan, name, *a, **kw: made.append(name))
+    packed, pos = Z(2, 4, 6, 64), Z(1, 2, 4, dtype=torch.int32)
+    q, k, new = packed[:, :, :4], packed[:, :, 4:], lambda n: Z(2, 4, n, 64)
+    for a, b, out in ((q, q, (q, new(4))), (q, packed[:, :, 3:5], (q, new(2))), (packed[:, :, 2:4], q, (new(2), q)), (q, packed[:, :, 1:2], (q, new(1)))):
+        with pytest.raises(ValueError):
+            ops.rope_axes(a, b, pos, Z(32), (32,), out=out)
+    assert not made
+    ops.rope_axes(q, k, pos, Z(32), (32,), out=(q, new(2)))
+    ops.rope_axes(q, k, pos, Z(32), (32,), out=(new(4), k))
+    ops.rope_axes(q, k, pos, Z(32), (32,), out=(q, k))
+    ops.rope_axes(q, None, pos, Z(32), (32,), out=(q, None))
+    assert made == ["smbv_rope_axes"] * 4
