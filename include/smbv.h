@@ -491,7 +491,8 @@ int smbv_vjepa_backward(const smbv_vjepa_cfg* cfg, const smbv_vjepa_tensors* par
  * j >= p - left or j < sinks); left / right < 0: unbounded; right = 0: causal.  q_lens / k_lens: int32 [B] on the device, clamped to [0, Sq] / [0, Sk], NULL:
  * Sq / Sk.  Rows that see nothing, padded rows included, get O = 0 and LSE = -inf and give no gradient; nothing past a length, and no key that no row of the
  * call can see, takes part, whatever it holds.  o_lo (optional, o's strides): the residual of o's rounding, from which the backward forms rowsum(dO * O).
- * lse: fp32 [B, H, Sq].  Pointers 16-byte aligned, strides multiples of 8.  The backward writes every element of dq, dk, dv. */
+ * lse: fp32 [B, H, Sq].  Pointers 16-byte aligned, strides multiples of 8, rows of k and v less than 2^24 elements apart.  The backward writes every element of
+ * dq, dk, dv. */
 typedef struct smbv_window_attn {
   int struct_bytes, dtype, B, Sq, Sk, H, Hk, Dh, left, right, sinks;
   float scale;                                /* > 0 */

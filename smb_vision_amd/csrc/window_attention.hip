@@ -407,7 +407,8 @@ int window_attention_check(const WinDesc& d, bool backward, const char* what, bo
       continue;
     }
     if (((uintptr_t)x.p & (x.align - 1)) || ((x.s->b | x.s->r | x.s->h) & 7)) { set_error("%s: %s must be 16-byte aligned with strides that are multiples of 8 elements", what, x.name); return SMBV_ERR_ALIGN; }
-    if (x.s->r >= (1 << 24) || x.s->h >= (1 << 24)) { set_error("%s: %s has rows or heads 2^24 elements apart", what, x.name); return SMBV_ERR_SHAPE; }   // (offsets inside a tile are 32-bit)
+    // (rows of keys and values inside a tile are reached by 32-bit offsets; everything else by 64-bit ones, to any distance that memory has)
+    if (x.s->r >= (x.s == &d.sk || x.s == &d.sv ? 1ll << 24 : 1ll << 40) || x.s->h >= (1ll << 40)) { set_error("%s: %s has its rows or heads too many elements apart", what, x.name); return SMBV_ERR_SHAPE; }
     if (x.s->b < 0 || x.s->r < 0 || x.s->h < 0) { set_error("%s: %s has a negative stride", what, x.name); return SMBV_ERR_SHAPE; }
   }
   if (!d.lse && d.B > 0 && d.Sq > 0) { set_error("%s: lse is null", what); return SMBV_ERR_ARG; }

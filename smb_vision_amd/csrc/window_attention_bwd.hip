@@ -186,6 +186,7 @@ __device__ __forceinline__ WinRun win_key_rows(const WinDesc& d, const WinSeq& s
 // few tiles to fill the chip); a tile's workgroups leave their fp32 sums in the workspace and a second launch adds them in order.
 struct WinSplit {
   int tiles, nsink, c1, c2, units;  // units: workgroups of one key head
+  int fixed;                        // the rows of a tile of 64 lie at 32-bit distances from its first, the same in every tile
   float* part;                      // [B, Hk][slots][dK | dV][BK keys][DP]
 };
 __device__ __host__ __forceinline__ int win_split_slots(const WinSplit& s) { return (s.c1 > 1 ? s.nsink * s.c1 : 0) + (s.c2 > 1 ? (s.tiles - s.nsink) * s.c2 : 0); }
@@ -246,7 +247,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     qoff[p] = (unsigned)(i * (unsigned)d.sq.r + g * (unsigned)d.sq.h) * 2 + copy.chunk[p] * 16;
     goff[p] = (unsigned)(i * (unsigned)d.sg.r + g * (unsigned)d.sg.h) * 2 + copy.chunk[p] * 16;
   }
-  const bool fixed = 64 % d.G == 0;   // (a tile then starts at a whole query, and its rows lie at fixed distances)
   const uint16_t* qb = d.q + b * d.sq.b + (long long)hk * d.G * d.sq.h;
   const uint16_t* gb = d.g + b * d.sg.b + (long long)hk * d.G * d.sg.h;
   // the rows' numbers travel with the tile: wave 0 copies the LSEs, wave 1 the deltas, wave 2 the exponents (256 bytes; a count that is the same in all waves
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((int)lds_addr_of(smem)), lds = lds0 + w * (IMG / NW), lds_num = lds0 + STAT + 256 * min(w, 3);
   auto stage = [&](int j, int slot) __attribute__((always_inline)) {
     const int q0 = rlo + 64 * j;
-    if (fixed && q0 + 64 <= rhi) {
+    if (sp.fixed && q0 + 64 <= rhi) {
       const int i = win_div(d, q0);
       const uint16_t *qs = win_uniform(qb + (long long)i * d.sq.r), *gs = win_uniform(gb + (long long)i * d.sg.r);
 #pragma unroll
@@ -443,8 +443,13 @@ __global__ __launch_bounds__(256) void win_dkv_join_kernel(WinDesc d, WinSplit s
 
 static constexpr int WIN_BK = 128;   // keys a workgroup (4 waves of 32)
 static int win_dp(const WinDesc& d) { return d.D <= 32 ? 32 : d.D <= 64 ? 64 : 128; }
+// (a tile that starts at a whole query; long head-major operands have their heads further apart than 32 bits reach)
+static bool win_fixed(const WinDesc& d, const WinStride& s) {
+  return 64 % d.G == 0 && (64 / d.G - 1) * s.r + (d.G - 1) * s.h < (1ll << 30) - 128;
+}
 static WinSplit win_split(const WinDesc& d) {
   WinSplit s = {};
+  s.fixed = win_fixed(d, d.sq) && win_fixed(d, d.sg);
   const int bk = WIN_BK;
   s.tiles = (d.Sk + bk - 1) / bk;
   s.nsink = d.left < 0 ? 0 : std::min(s.tiles, (int)(((long long)std::min(d.sinks, d.Sk) + bk - 1) / bk));

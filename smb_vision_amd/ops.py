@@ -468,8 +468,8 @@ def _window_args(q, k, v, left, right, sinks, scale, q_lens, k_lens):
 def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_lens=None, k_lens=None, resid=False, out=None):
     """Softmax attention inside a sliding window, with a few first tokens that stay visible (smbv_window_attention_fwd).
 
-    q [B, Sq, H, D], k / v [B, Sk, Hk, D] (bf16 or fp16, any batch / row / head strides that are multiples of 8 elements, H a multiple of Hk, D a multiple of 8
-    up to 128).  Query i stands at position p = i + k_len - q_len and sees key j iff j < k_len, j <= p + right (right < 0: no bound; 0: causal) and
+    q [B, Sq, H, D], k / v [B, Sk, Hk, D] (bf16 or fp16, any batch / row / head strides that are multiples of 8 elements - rows of k and v less than 2^24
+    elements apart -, H a multiple of Hk, D a multiple of 8 up to 128).  Query i stands at position p = i + k_len - q_len and sees key j iff j < k_len, j <= p + right (right < 0: no bound; 0: causal) and
     (j >= p - left (left < 0: no bound) or j < sinks).  q_lens / k_lens: int32 [B] on the device (None: Sq / Sk), so the queries are the last rows of their
     sequence: all of them in training, the newest tokens against a cache in serving (Sq = 1; the whole cache with k_lens keeps the call's signature).  A row that sees nothing, padded rows included, is 0 with lse -inf.
     Keys that no row of a call can see do not take part, whatever they hold; a NaN or infinity in a value that SOME rows see can reach other rows near them.

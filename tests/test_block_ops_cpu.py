@@ -297,3 +297,16 @@ def test_turned_in_place_beside_an_operand_that_is_still_read(dry, monkeypatch):
     ops.rope_axes(q, k, pos, Z(32), (32,), out=(q, k))
     ops.rope_axes(q, None, pos, Z(32), (32,), out=(q, None))
     assert made == ["smbv_rope_axes"] * 4
+
+
+def test_heads_may_lie_far_apart():
+    """Head-major operands [B, H, S, D] of any length: the call gets as far as its workspace (too small here, so nothing is launched)."""
+    lib = _lib.load()
+    for S, D in ((1 << 17, 128), (1 << 18, 64), (1 << 22, 128)):
+        q, k = _lib.c_ll3(4 * S * D, D, S * D), _lib.c_ll3(2 * S * D, D, S * D)
+        a = attn(B=1, Sq=S, Sk=S, Dh=D, sq=q, so=q, sdo=q, sdq=q, sk=k, sv=k, sdk=k, sdv=k)
+        assert lib.smbv_window_attention_bwd(C.byref(a), P, 256, None) == -4, _lib.last_error()
+        a.Sq, a.H, a.left = 1, 8, -1   # one token: the shares of its keys need a workspace
+        assert lib.smbv_window_attention_fwd(C.byref(a), P, 256, None) == -4, _lib.last_error()
+    for far in (dict(sk=_lib.c_ll3(0, 1 << 24, 64)), dict(sv=_lib.c_ll3(0, 1 << 24, 64)), dict(sq=_lib.c_ll3(0, 256, 1 << 40)), dict(so=_lib.c_ll3(0, 1 << 40, 64))):
+        assert lib.smbv_window_attention_fwd(C.byref(attn(**far)), P, 1 << 40, None) == -1 and "apart" in _lib.last_error()

@@ -366,3 +366,32 @@ def test_a_cache_beyond_32_bit_offsets(ops):
             if left > 0:
                 do = torch.randn_like(q)
                 assert all(torch.equal(a, b) for a, b in zip(ops.window_attention_bwd(q, k, v, o, do, lse, **kw), ops.window_attention_bwd(q, kb, vb, o, do, lse, **kw)))
+
+
+def apart(t, gap):
+    """t [B, S, H, D] as a head-major view whose heads lie `gap` elements apart."""
+    B, S, H, D = t.shape
+    buf = torch.empty((H - 1) * gap + B * S * D, dtype=t.dtype, device="cuda")
+    return buf.as_strided((B, S, H, D), (S * D, D, gap, 1)).copy_(t)
+
+
+@pytest.mark.parametrize("H,Hk,gap", [(2, 1, 2 ** 31 + 64), (8, 8, 2 ** 24 + 8), (4, 1, 2 ** 28)])
+def test_heads_far_apart(ops, H, Hk, gap):
+    """Head-major operands with 2^24 elements and more between the heads (caches of 131,072 keys of 128 channels and longer), beyond 32-bit offsets too."""
+    B, S, D = 1, 300, 64
+    q, k, v = operands(BF, B, S, S, H, Hk, D)
+    do = torch.randn(B, S, H, D, generator=torch.Generator().manual_seed(9)).to(BF).cuda()
+    kw = dict(left=60, right=0, sinks=3)
+    o, lse = ops.window_attention_fwd(q, k, v, **kw)
+    want = ops.window_attention_bwd(q, k, v, o, do, lse, **kw)
+    fq, fk, fv, fdo = (apart(t, gap) for t in (q, k, v, do))
+    o2, lse2 = ops.window_attention_fwd(fq, fk, fv, **kw)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    assert all(torch.equal(a, b) for a, b in zip(want, ops.window_attention_bwd(fq, fk, fv, o2, fdo, lse2, **kw)))
+    outs = [apart(torch.zeros_like(t), gap) for t in (q, k, v)]
+    fo = apart(torch.zeros_like(o), gap)
+    ops.window_attention_fwd(fq, fk, fv, out=fo, **kw)
+    ops.window_attention_bwd(fq, fk, fv, fo, fdo, lse, out=outs, **kw)
+    assert torch.equal(fo, o) and all(torch.equal(a, b) for a, b in zip(want, outs))
+    for t in (1, 7):   # few rows: the other forward kernel
+        assert torch.equal(ops.window_attention_fwd(fq[:, :t], fk, fv, **kw)[0], ops.window_attention_fwd(q[:, :t], k, v, **kw)[0])
