@@ -7,9 +7,11 @@
 //             head's queries is formed: S and dP by one product each, dV^T += dO^T P, dK^T += Q^T dS
 // S and dP are formed twice (7 products instead of 5): the alternative is dQ by float atomics, whose order changes the result.
 // P and dS are rounded to 16 bits for the second products, which add in 32 bits.  fp16 has a narrow exponent: gradients of 2^-20 would be lost in dS.  So dS is
-// formed in units of a power of two: dQ's wave takes dO times 2^-e, e the exponent of the row's largest |dO| (exact), dK's keeps its accumulator in
-// units of 2^e, e the largest exponent among the rows met so far, and rescales it when that grows.
+// formed in units of a power of two: dQ's wave takes dO times 2^-e, e the exponent of the row's largest |dO| (exact), dK's keeps a key's accumulator in
+// units of 2^e, e the largest exponent among the rows that the key has seen so far, and rescales it when that grows.  (Rows that it does not see do not count: one
+// with a gradient 2^24 times the others' would take all their digits.)
 #include "window_attention.h"
+#include <limits.h>
 #include <math.h>
 
 namespace smbv {
@@ -171,6 +173,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
     }
 }
 
+// the largest over the wave's lanes: prefix maxima inside rows of 16 lanes, then lane 15 of one row to the next, then lane 31 to the upper half
+__device__ __forceinline__ int win_wave_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The rows (r = i G + g) that see a key: [lo, hi), and all of them behind lo when it is a sink
 struct WinRun { int lo, hi; };
 __device__ __forceinline__ WinRun win_key_rows(const WinDesc& d, const WinSeq& s, int key) {
@@ -238,7 +251,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
   for (int dt = 0; dt < DT; dt++)
 #pragma unroll
     for (int x = 0; x < 16; x++) { dk[dt][x] = 0.f; dv[dt][x] = 0.f; }
-  int emax = WIN_NO_EXP;
+  int emax = WIN_NO_EXP, emin = WIN_NO_EXP;   // the exponent of this lane's key, and the least of the wave's keys
   const Copy copy(w, l, d.D);
   unsigned qoff[Copy::NP], goff[Copy::NP];
 #pragma unroll
@@ -287,16 +300,26 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
     const bool all = q0 >= all_lo && q0 + 64 <= all_hi;
     float unit = 1.f;
     if constexpr (E::half) {
-      int e = *(const int*)(st + 512 + 4 * l);
-      if (__builtin_amdgcn_ballot_w64(e > emax) != 0) {   // (seldom after the first tiles)
+      int er = *(const int*)(st + 512 + 4 * l);   // row q0 + l's
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(er > emin) != 0, 0)) {   // (seldom after the first tiles)
+        const int a = max(0, min(64, mine.lo - q0)), z = max(0, min(64, min(mine.hi, rhi) - q0));
+        const unsigned long long in = z > a ? (~0ull >> (64 - z + a)) << a : 0;   // the rows that this lane's key sees
+        int e = emax;
+        bool open = in != 0;
+        // the tile's exponents from the largest down, until every key has met one of its rows (every turn takes a row out)
+        for (int m = win_wave_max(er); m > WIN_NO_EXP && __builtin_amdgcn_ballot_w64(open) != 0; m = win_wave_max(er)) {
+          if ((in & __builtin_amdgcn_ballot_w64(er == m)) != 0) { e = max(e, m); open = false; }
+          if (er == m) er = WIN_NO_EXP;
+        }
+        if (__builtin_amdgcn_ballot_w64(e != emax && emax != WIN_NO_EXP) != 0) {   // (without an exponent nothing has been added yet)
+          const float f = emax == WIN_NO_EXP ? 1.f : ldexpf(1.f, emax - e);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 64));
-        const float f = emax == WIN_NO_EXP ? 0.f : ldexpf(1.f, emax - e);
+          for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-          for (int x = 0; x < 16; x++) dk[dt][x] *= f;
+            for (int x = 0; x < 16; x++) dk[dt][x] *= f;
+        }
         emax = e;
+        emin = -win_wave_max(key < seq.klen ? -e : -INT_MAX);
       }
       unit = emax == WIN_NO_EXP ? 1.f : ldexpf(1.f, -emax);
     }

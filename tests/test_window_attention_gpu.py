@@ -395,3 +395,26 @@ def test_heads_far_apart(ops, H, Hk, gap):
     assert torch.equal(fo, o) and all(torch.equal(a, b) for a, b in zip(want, outs))
     for t in (1, 7):   # few rows: the other forward kernel
         assert torch.equal(ops.window_attention_fwd(fq[:, :t], fk, fv, **kw)[0], ops.window_attention_fwd(q[:, :t], k, v, **kw)[0])
+
+
+@pytest.mark.parametrize("S,H,Hk,D,left,right,sinks", [(300, 2, 1, 64, 5, 0, 2), (200, 2, 2, 128, 20, 10, 0), (700, 3, 1, 32, 40, 0, 40), (130, 1, 1, 80, -1, 0, 0)])
+def test_fp16_gradients_beside_a_row_that_a_key_does_not_see(ops, S, H, Hk, D, left, right, sinks):
+    """One query's gradient is 2^24 times the others'.  The keys that it does not see keep their digits: their gradients are those of the call without it, bit
+    for bit, and within the definition's tolerance for that call."""
+    q, k, v = operands(HF, 1, S, S, H, Hk, D)
+    small = (torch.randn(1, S, H, D, generator=torch.Generator().manual_seed(8)) * 2.0 ** -13).to(HF).cuda()
+    kw = dict(left=left, right=right, sinks=sinks)
+    o, lse, lo = ops.window_attention_fwd(q, k, v, resid=True, **kw)
+    for at in (S // 3, S - 1):
+        big, none = small.clone(), small.clone()
+        big[:, at], none[:, at] = 2.0 ** 12, 0
+        seen = (torch.arange(S) <= at + right) if right >= 0 else torch.ones(S, dtype=torch.bool)
+        if left >= 0:
+            seen &= (torch.arange(S) >= at - left) | (torch.arange(S) < sinks)
+        g, g0 = ([t.clone() for t in ops.window_attention_bwd(q, k, v, o, d, lse, o_lo=lo, **kw)] for d in (big, none))
+        ref, _ = definition(q, k, v, none, left, right, sinks, D ** -0.5, None, None)
+        assert bool((~seen).any()) or at == S - 1
+        for n, a, b in zip("qkv", g, g0):
+            close(b, ref["d" + n], ref["t" + n], "d" + n)
+            if n != "q":
+                assert torch.equal(a[:, ~seen.cuda()], b[:, ~seen.cuda()]), (at, n)
