@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void win_rows_kernel(WinDesc d, WinRows wr) {
     const long long at = (((long long)b * d.Hk + hk) * d.Sq + i) * d.G + g;
     const float ls = live ? d.lse[((long long)b * d.H + h) * d.Sq + i] : -INFINITY;
     wr.lse2[at] = ls == -INFINITY ? INFINITY : ls * 1.4426950408889634f;
-    wr.ndelta[at] = -s;
+    wr.ndelta[at] = ls == -INFINITY ? 0.f : -s;   // (a row that sees nothing gives no gradient, whatever its dO holds)
     if constexpr (E::half) wr.expo[at] = mx > 0.f && mx < INFINITY ? ilogbf(mx) : WIN_NO_EXP;
   }
 }
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
       x = *(const u32x4*)(d.q + b * d.sq.b + i * d.sq.r + head * d.sq.h + ch);
       y = *(const u32x4*)(d.g + b * d.sg.b + i * d.sg.r + head * d.sg.h + ch);
     }
+    if (lse2 == INFINITY) { x = (u32x4){0, 0, 0, 0}; y = x; }   // the row sees nothing
     asm volatile("" : "+v"(x), "+v"(y));   // (waited for here, not in the loop)
     qf[ks] = __builtin_bit_cast(v8, x);
     gf[ks] = __builtin_bit_cast(v8, y);
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
       if (d0 >= d.D) continue;
       float a[4];
 #pragma unroll
-      for (int x = 0; x < 4; x++) a[x] = live ? acc[dt][4 * rg + x] * f : 0.f;
+      for (int x = 0; x < 4; x++) a[x] = lse2 != INFINITY ? acc[dt][4 * rg + x] * f : 0.f;
       *(u32x2*)(out + d0) = (u32x2){el_pack<E>(a[0], a[1]), el_pack<E>(a[2], a[3])};
     }
 }

@@ -418,3 +418,25 @@ def test_fp16_gradients_beside_a_row_that_a_key_does_not_see(ops, S, H, Hk, D, l
             close(b, ref["d" + n], ref["t" + n], "d" + n)
             if n != "q":
                 assert torch.equal(a[:, ~seen.cuda()], b[:, ~seen.cuda()]), (at, n)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_rows_that_see_nothing_give_no_gradient(ops, dtype, junk):
+    """More queries than keys: the first rows see nothing.  Whatever their query and their gradient hold, their dQ is 0 and no other gradient changes."""
+    B, Sq, Sk, H, Hk, D = 2, 90, 50, 4, 2, 64
+    q, k, v = operands(dtype, B, Sq, Sk, H, Hk, D)
+    do = (torch.randn(B, Sq, H, D, generator=torch.Generator().manual_seed(4)) * 0.1).to(dtype).cuda()
+    kl = torch.tensor([50, 31], dtype=torch.int32, device="cuda")
+    kw = dict(left=20, right=0, sinks=2, k_lens=kl)
+    o, lse, lo = ops.window_attention_fwd(q, k, v, resid=True, **kw)
+    want = ops.window_attention_bwd(q, k, v, o, do, lse, o_lo=lo, **kw)
+    q2, do2 = q.clone(), do.clone()
+    for b, n in enumerate((50, 31)):
+        assert bool((lse[b, :, :Sq - n] == -float("inf")).all()) and not bool(o[b, :Sq - n].any()) and not bool(want[0][b, :Sq - n].any())
+        q2[b, :Sq - n] = junk
+        do2[b, :Sq - n] = junk
+    o2, lse2, lo2 = ops.window_attention_fwd(q2, k, v, resid=True, **kw)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2) and torch.equal(lo, lo2)
+    for n, a, b in zip("qkv", want, ops.window_attention_bwd(q2, k, v, o2, do2, lse2, o_lo=lo2, **kw)):
+        assert torch.equal(a, b), n
