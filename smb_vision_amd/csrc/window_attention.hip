@@ -156,7 +156,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
     if (h2 == 0) *(float2*)(out + 32 * DP + 2 * r31) = make_float2(m2, sum);
     return;
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const bool some = live && sum != 0.f;   // (a row that sees nothing is 0, also beside an infinity in a value that others see)
+  const float inv = 1.0f / sum;
   if (r >= rows) return;
   const long long oo = b * d.so.b + i * d.so.r + head * d.so.h;
 #pragma unroll
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
       if (d0 >= d.D) continue;
       float f[4];
 #pragma unroll
-      for (int x = 0; x < 4; x++) f[x] = live ? ot[dt][4 * rg + x] * inv : 0.f;
+      for (int x = 0; x < 4; x++) f[x] = some ? ot[dt][4 * rg + x] * inv : 0.f;
       const u32x2 pk = {el_pack<E>(f[0], f[1]), el_pack<E>(f[2], f[3])};
       *(u32x2*)(d.o + oo + d0) = pk;
       if (d.o_lo) {
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
         *(u32x2*)(d.o_lo + oo + d0) = (u32x2){el_pack<E>(f[0], f[1]), el_pack<E>(f[2], f[3])};
       }
     }
-  if (h2 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !live || sum == 0.f ? -INFINITY : (m2 + __log2f(sum)) * 0.6931471805599453f;
+  if (h2 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !some ? -INFINITY : (m2 + __log2f(sum)) * 0.6931471805599453f;
 }
 
 // ---- few rows against many keys (single tokens) ------------------------------------------------------------------------------------------------------------
@@ -187,15 +188,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OC
 template <class E, int N>
 __device__ __forceinline__ void win_few_store(const WinDesc& d, const float (&o)[N], int ch0, int rr, int hk, int b, float m, float total, const WinSeq& seq) {
   const int i = win_div(d, rr), head = hk * d.G + (rr - i * d.G);
-  const bool live = i < seq.qlen;
-  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  const bool some = i < seq.qlen && total != 0.f;
+  const float inv = 1.0f / total;
   const long long oo = b * d.so.b + i * d.so.r + head * d.so.h + ch0;
 #pragma unroll
   for (int x = 0; x < N; x += 4) {
     if (ch0 + x >= d.D) continue;
     float f[4];
 #pragma unroll
-    for (int y = 0; y < 4; y++) f[y] = live ? o[x + y] * inv : 0.f;
+    for (int y = 0; y < 4; y++) f[y] = some ? o[x + y] * inv : 0.f;
     const u32x2 pk = {el_pack<E>(f[0], f[1]), el_pack<E>(f[2], f[3])};
     *(u32x2*)(d.o + oo + x) = pk;
     if (d.o_lo) {
@@ -204,7 +205,7 @@ __device__ __forceinline__ void win_few_store(const WinDesc& d, const float (&o)
       *(u32x2*)(d.o_lo + oo + x) = (u32x2){el_pack<E>(f[0], f[1]), el_pack<E>(f[2], f[3])};
     }
   }
-  if (ch0 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !live || total == 0.f ? -INFINITY : (m + __log2f(total)) * 0.6931471805599453f;
+  if (ch0 == 0) d.lse[((long long)b * d.H + head) * d.Sq + i] = !some ? -INFINITY : (m + __log2f(total)) * 0.6931471805599453f;
 }
 
 template <class E, int DP>

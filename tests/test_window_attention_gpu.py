@@ -440,3 +440,16 @@ def test_rows_that_see_nothing_give_no_gradient(ops, dtype, junk):
     assert torch.equal(o, o2) and torch.equal(lse, lse2) and torch.equal(lo, lo2)
     for n, a, b in zip("qkv", want, ops.window_attention_bwd(q2, k, v, o2, do2, lse2, o_lo=lo2, **kw)):
         assert torch.equal(a, b), n
+
+
+@pytest.mark.parametrize("Sq,Sk,H", [(90, 50, 2), (12, 5, 2), (40, 20, 1)])
+def test_rows_that_see_nothing_beside_infinite_values(ops, Sq, Sk, H):
+    """An infinity in a value that other rows of the tile see: the rows that see nothing are 0 with lse -inf, their dQ is 0."""
+    q, k, v = operands(BF, 1, Sq, Sk, H, 1, 64)
+    do = torch.ones_like(q)
+    v[:, :3] = float("inf")
+    kw = dict(left=20, right=0, sinks=1)
+    o, lse, lo = ops.window_attention_fwd(q, k, v, resid=True, **kw)
+    n = Sq - Sk
+    assert not bool(o[:, :n].any()) and not bool(lo[:, :n].any()) and bool((lse[:, :, :n] == -float("inf")).all()) and bool((lse[:, :, n:] > -float("inf")).all())
+    assert not bool(ops.window_attention_bwd(q, k, v, o, do, lse, o_lo=lo, **kw)[0][:, :n].any())
