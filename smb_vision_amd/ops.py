@@ -492,7 +492,7 @@ def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_l
     if out is None:
         o = plan.empty(0)
     else:
-        _writable(out, "out", (q, k, v))
+        _writable(out, "out", (q, k, v, q_lens, k_lens))
         o = out
     o_lo = _empty_strided(o.shape, o.stride(), dtype=o.dtype, device=device) if resid else None
     lse = plan.empty(1)
@@ -537,7 +537,7 @@ def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, sca
     else:
         dq, dk, dv = outs
         for name, t in zip(("dq", "dk", "dv"), outs):
-            _writable(t, name, (q, k, v, o, do, o_lo, lse))
+            _writable(t, name, (q, k, v, o, do, o_lo, lse, q_lens, k_lens))
         _apart(*outs)
     a = _lib.WindowAttn.from_buffer_copy(plan.args)
     a.q_lens, a.k_lens, a.q, a.k, a.v = _p(q_lens), _p(k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr()

@@ -310,3 +310,17 @@ def test_heads_may_lie_far_apart():
         assert lib.smbv_window_attention_fwd(C.byref(a), P, 256, None) == -4, _lib.last_error()
     for far in (dict(sk=_lib.c_ll3(0, 1 << 24, 64)), dict(sv=_lib.c_ll3(0, 1 << 24, 64)), dict(sq=_lib.c_ll3(0, 256, 1 << 40)), dict(so=_lib.c_ll3(0, 1 << 40, 64))):
         assert lib.smbv_window_attention_fwd(C.byref(attn(**far)), P, 1 << 40, None) == -1 and "apart" in _lib.last_error()
+
+
+def test_outputs_lie_apart_from_the_lengths(dry):
+    q, k, v = (Z(2, 4, n, 64, dtype=BF) for n in (2, 1, 1))
+    o, lse, fresh = q.clone(), Z(2, 2, 4), lambda: [t.clone() for t in (q, k, v)]
+    for name in ("q_lens", "k_lens"):
+        out = fresh()
+        lens = {name: out[0].view(-1)[8:12].view(torch.int32)}
+        with pytest.raises(ValueError, match="overlap"):
+            ops.window_attention_fwd(q, k, v, out=out[0], **lens)
+        for n in range(3):
+            out = fresh()
+            with pytest.raises(ValueError, match="overlap"):
+                ops.window_attention_bwd(q, k, v, o, o.clone(), lse, out=out, **{name: out[n].view(-1)[8:12].view(torch.int32)})
