@@ -58,8 +58,9 @@ class _SmbvAttentionFn(torch.autograd.Function):
 def smbv_attention(module, query, key, value, attention_mask=None, *, scaling=None, dropout=0.0, is_causal=False, **kwargs):
     """transformers attention-interface function (same contract as its `eager_attention_forward`): bf16 MFMA arithmetic, fp32 softmax
     statistics; returns (context [B, S, H, Dh] in the dtype of `query`, None)."""
-    if attention_mask is not None:
-        raise ValueError("smbv attention: attention / head masks are not supported (the reference's training path passes None)")
+    _refuse(kwargs)
+    if attention_mask is not None and not (isinstance(attention_mask, _WindowMask) and (attention_mask.left, attention_mask.right) == (-1, -1)):
+        raise ValueError("smbv attention: attention / head masks are not supported (the reference's training path passes None), nor is a model's causal or sliding one")
     if dropout:
         raise ValueError("smbv attention: attention dropout is not supported (the reference trains with attention_probs_dropout_prob = 0)")
     if is_causal:
@@ -69,7 +70,7 @@ def smbv_attention(module, query, key, value, attention_mask=None, *, scaling=No
                          f"{tuple(key.shape)}, {tuple(value.shape)}")
     if query.shape[-1] not in (64, 32):
         raise ValueError(f"smbv attention: head width {query.shape[-1]} has no native build (64 and 32 do)")
-    if not query.is_cuda:
+    if not _on_gpu(query):
         raise RuntimeError("smbv attention needs an MI355X: there is no CPU path")
     if scaling is None:
         scaling = query.shape[-1] ** -0.5
@@ -77,9 +78,11 @@ def smbv_attention(module, query, key, value, attention_mask=None, *, scaling=No
 
 
 def register(name=NAME):
-    """Make `config._attn_implementation = name` select the MI355X kernels (transformers.AttentionInterface)."""
-    from transformers import AttentionInterface
+    """Make `config._attn_implementation = name` select the MI355X kernels (transformers.AttentionInterface); a model's own masks raise
+    unless they show everything (transformers.AttentionMaskInterface)."""
+    from transformers import AttentionInterface, AttentionMaskInterface
     AttentionInterface.register(name, smbv_attention)
+    AttentionMaskInterface.register(name, _window_mask)
     return name
 
 
@@ -117,7 +120,7 @@ _HARMLESS = {"position_ids", "cache_position", "use_cache", "output_attentions",
 def _refuse(kwargs):
     for name, x in kwargs.items():
         if x is not None and name not in _HARMLESS:
-            raise ValueError(f"smbv window attention: the argument {name!r} is not supported (a cap on the scores, learned sinks, a bias: they change the result)")
+            raise ValueError(f"smbv attention: the argument {name!r} is not supported (a cap on the scores, learned sinks, a bias: they change the result)")
 
 
 def _on_gpu(t):
@@ -133,7 +136,7 @@ class _WindowMask:
         self.queries, self.keys, self.left, self.right, self.dropped = queries, keys, left, right, dropped
 
 
-_EMPTY_SLOTS = "smbv window attention: {} positions hold tokens and there are {} keys: no preallocated cache with empty slots"
+_EMPTY_SLOTS = "smbv attention: {} positions hold tokens and there are {} keys: no preallocated cache with empty slots"
 
 
 def _window_mask(*, batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function, attention_mask=None, device=None, **unused):
@@ -144,11 +147,11 @@ def _window_mask(*, batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
     n, m, q0, k0 = int(q_length), int(kv_length), int(q_offset), int(kv_offset)
     if attention_mask is not None:
         if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("smbv window attention: a padding mask cannot be looked at inside a graph capture; pass none (every position holds a token)")
+            raise RuntimeError("smbv attention: a padding mask cannot be looked at inside a graph capture; pass none (every position holds a token)")
         if attention_mask.shape[-1] < k0 + m:
             raise ValueError(_EMPTY_SLOTS.format(attention_mask.shape[-1], k0 + m))
         if attention_mask.dim() != 2 or not bool(attention_mask[:, k0:k0 + m].all()):
-            raise ValueError("smbv window attention: padded batches are not supported (every position of the attention mask has to hold a token); "
+            raise ValueError("smbv attention: padded batches are not supported (every position of the attention mask has to hold a token); "
                              "ops.window_attention_fwd takes per-sequence lengths")
 
     def sees(dev, qi, kj):
@@ -184,7 +187,7 @@ def _window_mask(*, batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
     if found != (-1, -1) and q0 - k0 != m - n:
         raise ValueError(_EMPTY_SLOTS.format(q0 - k0 + n, m))
     if found is None:
-        raise ValueError("smbv window attention: the model's mask is no sliding window over full sequences (packed documents, blocks and prefixes are not supported)")
+        raise ValueError("smbv attention: the model's mask is no sliding window over full sequences (packed documents, blocks and prefixes are not supported)")
     return _WindowMask(n, m, *found, k0)
 
 

@@ -213,3 +213,27 @@ def test_forward_mode_tangents_are_not_dropped(calls, grad):
     assert not o.requires_grad and o.grad_fn is None
     with torch.no_grad():
         assert torch.equal(attention_plugin.smbv_window_attention(m, x.clone().requires_grad_(True), x, x)[0], o)
+
+
+def test_full_attention_by_name_refuses_other_masks(monkeypatch):
+    """The name "smbv" computes attention of everything to everything: a model that asks for less raises, and one that does not gets what eager gives."""
+    monkeypatch.setattr(attention_plugin, "_on_gpu", lambda t: True)
+    monkeypatch.setattr(attention_plugin._SmbvAttentionFn, "apply", lambda q, k, v, scale: definition(*(t.transpose(1, 2) for t in (q, k, v)), scale=scale)[0])
+    name = attention_plugin.register("smbv_for_test")
+    import transformers as t
+    base = dict(vocab_size=50, hidden_size=128, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2, attn_implementation=name)
+    bert = t.BertModel(t.BertConfig(**base)).eval()
+    ref = t.BertModel(t.BertConfig(**{**base, "attn_implementation": "eager"})).eval()
+    ref.load_state_dict(bert.state_dict())
+    for mask in (None, ONES):
+        assert rms_err(out(bert, IDS, attention_mask=mask), out(ref, IDS, attention_mask=mask)) < 1e-5
+    mask = ONES.clone()
+    mask[1, :3] = 0
+    with pytest.raises(ValueError, match="padded"):
+        out(bert, IDS, attention_mask=mask)
+    llama = t.LlamaForCausalLM(t.LlamaConfig(**base)).eval()
+    with pytest.raises(ValueError, match="causal"):
+        out(llama, IDS)
+    q = torch.zeros(1, 2, 8, 64)
+    with pytest.raises(ValueError, match="softcap"):
+        attention_plugin.smbv_attention(torch.nn.Module(), q, q, q, softcap=50.0)
