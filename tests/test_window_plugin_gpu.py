@@ -162,3 +162,50 @@ def test_a_block_of_them():
     got = (x2, y2, b1["dx"], b1["dh"], dwq, dwo, b1["post_w"], b1["pre_w"], b2["post_w"], b2["pre_w"], b1["gate"], b2["gate"])
     for n, a, b in zip(("x2", "y2", "dx", "dh", "dwq", "dwo", "dw1", "dw2", "dw3", "dw4", "dg1", "dg2"), got, (X2, Y2, *grads)):
         assert rms_err(a, b) < 1.1e-2, (n, rms_err(a, b))
+
+
+@pytest.mark.parametrize("kind", ["mistral", "llama"])
+def test_causal_models_by_name(kind):
+    """Mistral (a sliding window and a sliding cache) and Llama by name: a prompt, its gradients, and token by token, against their eager attention in fp32.
+    Tolerances as above for a whole model under bf16 operands: 2e-2 of the logits, 3e-2 of the gradients (rms)."""
+    import transformers as t
+    from smb_vision_amd import attention_plugin
+    name = attention_plugin.register_window()
+    base = dict(vocab_size=64, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2)
+    make = {"mistral": lambda a: t.MistralForCausalLM(t.MistralConfig(**base, sliding_window=24, attn_implementation=a)),
+            "llama": lambda a: t.LlamaForCausalLM(t.LlamaConfig(**base, attn_implementation=a))}[kind]
+    torch.manual_seed(0)
+    ref, ours = make("eager").cuda().train(), make(name).cuda().train()
+    ours.load_state_dict(ref.state_dict())
+    ids = torch.randint(0, 64, (2, 70), generator=torch.Generator().manual_seed(2)).cuda()
+    outs = [m(ids, attention_mask=torch.ones_like(ids), labels=ids) for m in (ref, ours)]
+    for o in outs:
+        o.loss.backward()
+    assert rms_err(outs[1].logits, outs[0].logits) < 2e-2
+    pr, po = dict(ref.named_parameters()), dict(ours.named_parameters())
+    worst = max((rms_err(po[n].grad, pr[n].grad), n) for n in pr)
+    assert worst[0] < 3e-2, worst
+    ours.eval()
+    cache, got = None, []
+    with torch.no_grad():
+        for n, at in ((40, 0), *((1, i) for i in range(40, 70))):
+            o = ours(ids[:, at:at + n], past_key_values=cache, use_cache=True)
+            cache = o.past_key_values
+            got.append(o.logits)
+    assert rms_err(torch.cat(got, 1), outs[0].logits) < 2e-2
+    mask = torch.ones_like(ids)
+    mask[1, :5] = 0
+    with pytest.raises(ValueError):
+        ours(ids, attention_mask=mask)
+
+
+def test_mask_that_looks_something_up_on_the_device():
+    """Packed documents are a table on the model's device: looked up there, and refused."""
+    from smb_vision_amd import attention_plugin
+    doc = torch.tensor([0] * 6 + [1] * 14, device="cuda")
+    kw = dict(batch_size=2, q_length=20, kv_length=20, dtype=BF, config=None, device=torch.device("cuda"))
+    with pytest.raises(ValueError):
+        attention_plugin._window_mask(mask_function=lambda b, h, q, k: (k <= q) & (doc[q] == doc[k]), **kw)
+    one = torch.zeros(20, dtype=torch.long, device="cuda")
+    m = attention_plugin._window_mask(mask_function=lambda b, h, q, k: (k <= q) & (one[q] == one[k]), **kw)
+    assert (m.left, m.right) == (-1, 0)
