@@ -492,7 +492,7 @@ int smbv_vjepa_backward(const smbv_vjepa_cfg* cfg, const smbv_vjepa_tensors* par
  * Sq / Sk.  Rows that see nothing, padded rows included, get O = 0 and LSE = -inf and give no gradient; nothing past a length, and no key that no row of the
  * call can see, takes part, whatever it holds.  o_lo (optional, o's strides): the residual of o's rounding, from which the backward forms rowsum(dO * O).
  * lse: fp32 [B, H, Sq].  Pointers 16-byte aligned, strides multiples of 8, rows of k and v less than 2^24 elements apart.  The backward writes every element of
- * dq, dk, dv. */
+ * dq, dk, dv.  In fp16 it holds dS in units of the largest |d_o| of a row, for dk of the rows that a key sees: |v| up to 16000 / Dh never overflows it. */
 typedef struct smbv_window_attn {
   int struct_bytes, dtype, B, Sq, Sk, H, Hk, Dh, left, right, sinks;
   float scale;                                /* > 0 */

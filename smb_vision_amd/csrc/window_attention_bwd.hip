@@ -481,7 +481,8 @@ static WinSplit win_split(const WinDesc& d) {
   const long long all = (long long)d.Sq * d.G, window = d.left < 0 || d.right < 0 ? all : std::min<long long>(all, ((long long)d.left + d.right + bk) * d.G);
   const long long plain = (long long)(s.tiles - s.nsink) * d.Hk * d.B;
   // A share costs its sums' way through memory (128 KiB at 128 keys of 128 channels, out and back) and saves a part of its tile's rows, a microsecond or two for
-  // 64 of them: no share has less than 1024 rows, and tiles are split only as far as there is room for more workgroups (two a CU; the sinks' four)
+  // 64 of them: no share has less than 1024 rows, and tiles are split only as far as there is room for more workgroups (counted as two a CU, though one fits at
+  // 128 channels; the sinks' four)
   s.c2 = (int)std::max<long long>(1, std::min<long long>({512 / std::max<long long>(plain, 1), window / 1024, 64}));
   const long long share = std::max<long long>(1024, (window + s.c2 - 1) / s.c2), sinks = (long long)s.nsink * d.Hk * d.B;
   s.c1 = (int)std::max<long long>(1, std::min<long long>({(all + share - 1) / share, 1024 / std::max<long long>(sinks, 1), 64}));

@@ -472,7 +472,8 @@ def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_l
     elements apart -, H a multiple of Hk, D a multiple of 8 up to 128).  Query i stands at position p = i + k_len - q_len and sees key j iff j < k_len, j <= p + right (right < 0: no bound; 0: causal) and
     (j >= p - left (left < 0: no bound) or j < sinks).  q_lens / k_lens: int32 [B] on the device (None: Sq / Sk), so the queries are the last rows of their
     sequence: all of them in training, the newest tokens against a cache in serving (Sq = 1; the whole cache with k_lens keeps the call's signature).  A row that sees nothing, padded rows included, is 0 with lse -inf.
-    Keys that no row of a call can see do not take part, whatever they hold; a NaN or infinity in a value that SOME rows see can reach other rows near them.
+    Keys that no row of a call can see do not take part, whatever they hold; a NaN or infinity in a value that SOME rows see can reach other rows near them that
+    see something.
 
     Returns (o [B, Sq, H, D], lse fp32 [B, H, Sq]) and with ``resid`` also the residual of o's rounding, which window_attention_bwd takes as ``o_lo``.
     out: a tensor for o (its strides free; with ``resid`` the residual gets a tensor of the same strides)."""
@@ -504,8 +505,9 @@ def window_attention_fwd(q, k, v, *, left=-1, right=-1, sinks=0, scale=None, q_l
 
 def window_attention_bwd(q, k, v, o, do, lse, *, left=-1, right=-1, sinks=0, scale=None, q_lens=None, k_lens=None, o_lo=None, out=None):
     """Gradients (dq, dk, dv) of window_attention_fwd (the same keyword arguments; o, lse and o_lo as it returned them; do: the gradient of o, any strides).
-    A key head's gradient is the sum over its query heads.  Every element is written; the same call gives the same bits.  out: three tensors for the
-    gradients, for instance the column blocks of one packed gradient."""
+    A key head's gradient is the sum over its query heads.  Every element is written; the same call gives the same bits.  In fp16, |v| above 16000 / D with
+    signs that agree can overflow (dS is held in units of the largest |do|).  out: three tensors for the gradients, for instance the column blocks of one
+    packed gradient."""
     left, right, sinks, scale = int(left), int(right), int(sinks), None if scale is None else float(scale)
     outs = (None,) * 3 if out is None else tuple(out)
     key = ("window_bwd", _meta(q), _meta(k), _meta(v), _meta(o), _meta(do), _meta(lse), left, right, sinks, scale, _meta(q_lens), _meta(k_lens), _meta(o_lo),
